@@ -49,6 +49,11 @@
  *   tf_prefill_attention     prefill's causal attention (runtime/prefill.py:84-88, 109-118)
  *   tf_argmax_rows           greedy sampling, torch.argmax(logits, dim=-1)
  *                            (scheduler/continuous.py:265-275)
+ *   tf_paged_kv_write_token_q8, tf_paged_kv_read_token_q8, tf_paged_gqa_decode_q8
+ *                            the 8-bit paged cache and attention over it (no
+ *                            counterpart in the reference)
+ *   tf_linear_mxfp4          a decode projection by 4-bit weights (no counterpart)
+ *   tf_token_logprobs        log probabilities, entropy and top tokens (no counterpart)
  *   tf_hbm_read_probe        measurement only: the read-rate ceiling the attention
  *                            roofline is compared with (the reference measures
  *                            its ceiling with a device copy,
@@ -124,7 +129,8 @@ enum tf_attention_variant {
 /* Message describing the last failure on the calling thread ("" if none). */
 const char *tf_last_error(void);
 
-/* Version of this ABI; bumped on any signature change or added entry point. */
+/* Version of this ABI; bumped on any change that existing callers have to follow (entry points
+ * may be added within a version). */
 int32_t tf_abi_version(void);
 
 /* Which kernel family tf_paged_gqa_decode uses for these parameters
@@ -650,6 +656,97 @@ typedef struct tf_prefill_layer_args {
   int32_t dtype;
 } tf_prefill_layer_args;
 int32_t tf_prefill_layer(const tf_prefill_layer_args *args, void *stream);
+
+/*
+ * The 8-bit paged KV cache.
+ *   key_cache    [num_blocks, kv_heads, block_size, head_dim] e4m3 codes
+ *   value_cache  [num_blocks, kv_heads, head_dim, block_size] e4m3 codes
+ *   key/value_scales [num_blocks, kv_heads] e8m0 bytes: a code of the page and
+ *                head stands for code * 2^(byte - 127), byte in 1..254
+ * head_dim is a multiple of 16 up to 256, block_size a multiple of 16 up to
+ * 1024, both caches 16-byte aligned.  No counterpart in the reference, whose
+ * cache holds 16- or 32-bit elements.
+ *
+ * tf_paged_kv_write_token_q8 appends rows of keys/values [rows, kv_heads,
+ * head_dim] at (physical_blocks[r], block_offsets[r]) where active_mask[r] !=
+ * 0; rows whose slot lies outside the cache are skipped.  Neighbouring rows
+ * at ascending offsets of one page form a run, and a page takes at most one
+ * run per call (two would race for its scale).  With t the smallest integer
+ * >= -126 such that max |finite x| <= 448 * 2^t over a run and head: a run
+ * from offset 0 begins its page, whose scale becomes 2^t (what the page held
+ * is void); any other raises the page's scale to 2^t if that is larger, the
+ * page's codes being rounded to the new one.  Codes round to nearest even;
+ * infinities and NaN are stored as NaN.
+ */
+int32_t tf_paged_kv_write_token_q8(
+    const void *keys, const void *values, void *key_cache, void *value_cache,
+    void *key_scales, void *value_scales, const int32_t *physical_blocks,
+    const int32_t *block_offsets, const int32_t *active_mask, int32_t rows,
+    int32_t kv_heads, int32_t head_dim, int32_t num_blocks, int32_t block_size,
+    int32_t dtype, void *stream);
+
+/*
+ * Token rows of the 8-bit cache as values: keys/values [rows, kv_heads,
+ * head_dim] (one rounding to dtype, none for bf16 and fp32) of the slots
+ * (physical_blocks[r], block_offsets[r]); zeros where a slot lies outside the
+ * cache.
+ */
+int32_t tf_paged_kv_read_token_q8(
+    const void *key_cache, const void *value_cache, const void *key_scales,
+    const void *value_scales, const int32_t *physical_blocks,
+    const int32_t *block_offsets, void *keys, void *values, int32_t rows,
+    int32_t kv_heads, int32_t head_dim, int32_t num_blocks, int32_t block_size,
+    int32_t dtype, void *stream);
+
+/*
+ * tf_paged_gqa_decode over the 8-bit cache: query, block_tables,
+ * context_lengths, output, partial buffers and scale as there (pages outside
+ * the cache are skipped, rows of no token are zeros), split_size a multiple of
+ * 64.  Several partitions are merged by a second launch.  Calls sharing
+ * partial buffers must not overlap in time.
+ */
+int32_t tf_paged_gqa_decode_q8(
+    const void *query, const void *key_cache, const void *value_cache,
+    const void *key_scales, const void *value_scales,
+    const int32_t *block_tables, const int32_t *context_lengths, void *output,
+    float *partial_max, float *partial_sum, float *partial_accumulator,
+    int64_t partial_capacity, int32_t partial_row_stride, int32_t batch,
+    int32_t query_heads, int32_t kv_heads, int32_t head_dim,
+    int32_t num_blocks, int32_t block_size, int32_t table_width,
+    int32_t split_size, int32_t num_splits, float scale, int32_t dtype,
+    void *stream);
+
+/*
+ * Decode-shaped linear layer by 4-bit weights, m <= 64 rows of fp16 or bf16:
+ *   y[r][j] = sum_k x[r][k] * e2m1(code[j][k]) * 2^(scale[j][k / 32] - 127)
+ * summed in fp32 and rounded once; with a residual (NULL: none),
+ * round(round(sum) + residual[r][j]).  weight [n, k / 2] holds two codes a
+ * byte, the even column in the low half (e2m1: sign bit 8, then 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6); scales [n, k / 32] are e8m0 bytes in 1..254.  k is a
+ * multiple of 32; x and weight rows are 16-byte aligned.  Strides count
+ * elements (bytes for weight and scales).  y may be residual itself, and
+ * overlaps no other input.
+ */
+int32_t tf_linear_mxfp4(const void *x, int64_t x_row_stride, const void *weight,
+                        int64_t weight_row_stride, const void *scales,
+                        int64_t scale_row_stride, const void *residual,
+                        int64_t residual_row_stride, void *y, int64_t y_row_stride,
+                        int32_t m, int32_t n, int32_t k, int32_t dtype, void *stream);
+
+/*
+ * Log probabilities of given tokens: per row r of logits (row_stride elements
+ * apart), with log p = log_softmax(row) in fp32:
+ *   logprobs[r] = log p(tokens[r]) (NaN where the token is outside the row)
+ *   entropy[r]  = -sum p log p (terms of p = 0 are 0)
+ *   top_tokens / top_logprobs [rows, top_k]: the top_k largest logits in
+ *   descending order, equal ones by index, a NaN above every number, and
+ *   their log p.
+ * top_k <= min(32, columns), 0 for none (the pointers may then be NULL).
+ */
+int32_t tf_token_logprobs(const void *logits, int64_t row_stride, int32_t rows, int32_t columns,
+                          const int64_t *tokens, float *logprobs, float *entropy,
+                          float *top_logprobs, int64_t *top_tokens, int32_t top_k,
+                          int32_t dtype, void *stream);
 
 /*
  * Measurement only: stream `bytes` (a positive multiple of 16) of the

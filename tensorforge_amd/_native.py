@@ -150,6 +150,24 @@ SIGNATURES: dict[str, tuple[Any, ...]] = {
         _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p,  # batch .. block size, dtype, stream
     ),
     "tf_prefill_layer": (ctypes.POINTER(PrefillLayerArgs), _p),
+    "tf_paged_kv_write_token_q8": (
+        _p, _p, _p, _p, _p, _p, _p, _p, _p,  # keys, values, caches, scales, pages, offsets, active
+        _i32, _i32, _i32, _i32, _i32, _i32, _p,  # rows .. block size, dtype, stream
+    ),
+    "tf_paged_kv_read_token_q8": (
+        _p, _p, _p, _p, _p, _p, _p, _p,  # caches, scales, pages, offsets, keys, values
+        _i32, _i32, _i32, _i32, _i32, _i32, _p,  # rows .. block size, dtype, stream
+    ),
+    "tf_paged_gqa_decode_q8": (
+        _p, _p, _p, _p, _p, _p, _p, _p,  # query, caches, scales, tables, lengths, output
+        _p, _p, _p, _i64, _i32,  # partials, capacity, row stride
+        _i32, _i32, _i32, _i32,  # batch, query heads, kv heads, head dim
+        _i32, _i32, _i32,  # num blocks, block size, table width
+        _i32, _i32, _f32, _i32, _p,  # split size, splits, scale, dtype, stream
+    ),
+    "tf_linear_mxfp4": (_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32,
+                        _p),
+    "tf_token_logprobs": (_p, _i64, _i32, _i32, _p, _p, _p, _p, _p, _i32, _i32, _p),
     "tf_prefill_attention": (_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _i32, _i32, _i32,
                              _f32, _i32, _i32, _p),
 }
@@ -239,6 +257,10 @@ def current_stream(device: torch.device) -> int:
 
     index = device.index
     return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+# Index of the current device, as cheap as the stream's handle above.
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def dtype_code(dtype: torch.dtype) -> int:

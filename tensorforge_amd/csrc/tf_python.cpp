@@ -108,6 +108,11 @@ PyMethodDef methods[] = {
     TF_ENTRY(tf_prefill_linear),
     TF_ENTRY(tf_prefill_linear_splits),
     TF_ENTRY(tf_prefill_layer),
+    TF_ENTRY(tf_paged_kv_write_token_q8),
+    TF_ENTRY(tf_paged_kv_read_token_q8),
+    TF_ENTRY(tf_paged_gqa_decode_q8),
+    TF_ENTRY(tf_linear_mxfp4),
+    TF_ENTRY(tf_token_logprobs),
     {nullptr, nullptr, 0, nullptr},
 };
 
