@@ -180,6 +180,18 @@ def test_nan_query_and_nan_codes_stay_in_their_rows(device):
     assert got[2, :4, 9].isnan().all() and int(got.isnan().sum()) == 4
 
 
+def test_nan_query_over_many_partitions(device):
+    """Every score of one head NaN in every partition."""
+
+    lengths = [3000]
+    reference = _reference(190, 2, 16, 64, seed=28)
+    tables = _tables(lengths, 16, 190, seed=28)
+    query = _query(1, 8, 64, torch.bfloat16, seed=29)
+    query[0, 5] = float("nan")
+    got = _run(device, reference, query, tables, lengths)
+    assert got[0, 5].isnan().all() and int(got.isnan().sum()) == 64
+
+
 @pytest.mark.parametrize("held", [1, 2, 5, 64])
 def test_workspace_and_output_are_used(device, held):
     """Fewer partitions where the workspace holds fewer; the same result within
