@@ -96,11 +96,18 @@ __device__ __forceinline__ void load_lds16(const void *src, uint32_t lds) {
 
 // The same from `base` + each lane's offset.  `base` must come from scalar
 // instructions: one that a vector instruction wrote needs five wait states.
+template <bool NT = false>
 __device__ __forceinline__ void load_lds16(const void *base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %0"
-               :
-               : "s"(base), "v"(offset), "{m0}"(lds)
-               : "memory");
+  if constexpr (NT)
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %0 nt"
+                 :
+                 : "s"(base), "v"(offset), "{m0}"(lds)
+                 : "memory");
+  else
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %0"
+                 :
+                 : "s"(base), "v"(offset), "{m0}"(lds)
+                 : "memory");
 }
 
 // ---------------------------------------------------------------------------

@@ -25,6 +25,10 @@
 // (times log2 e), the sum l of exp2(s - m) and the unnormalised output; the
 // wavefronts' meet in LDS.  Several partitions per row leave (m, l, numerator)
 // for tf_paged_gqa_decode_merge.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
 #include "tf_common.hpp"
 #include "tf_q8.hpp"
 
@@ -108,117 +112,74 @@ __device__ __forceinline__ float over_quads(float v, F combine) {
 
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 
-// What a wavefront loads of 64 tokens.
-template <int DMAX>
-struct Block {
-  u32x4 k[4][DMAX / 64];
-  u32x4 v[DMAX / 16];
-  uint32_t k_scale, v_scale;
-  int32_t tokens;  // of this lane's tile that count
+// One workgroup's part of a call: query heads [qh0, qh0 + heads) of row b, the
+// tokens [begin, end) of a partition.
+struct Part {
+  int32_t b, h, qh0, heads, begin, end, split;
 };
 
-// DMAX: head_dim, or with GUARD any head_dim up to it.
-template <typename T, int DMAX, bool GUARD>
-__global__ void __launch_bounds__(512) paged_decode_q8_kernel(Q8Params p) {
-  constexpr int PARTS = kParts<T>;
-  constexpr int KU = DMAX / 64;  // 16-byte loads of a key: 64 dimensions each
-  constexpr int DT = DMAX / 16;  // tiles of the output
-  constexpr bool AHEAD = DMAX <= 128;  // the next block is loaded before this one is used
-  extern __shared__ float merged[];    // [wavefronts][heads][D + 4]
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int waves = blockDim.x >> 6;
-  const int col = lane & 15;
-  const int quad = lane >> 4;
-  const int32_t D = GUARD ? p.head_dim : DMAX;
+__device__ __forceinline__ Part part_of(const Q8Params &p) {
+  Part w;
   const int32_t head_tiles = (p.group + 15) / 16;
-  const int32_t h = blockIdx.x / head_tiles;
-  const int32_t g0 = (blockIdx.x - h * head_tiles) * 16;
-  const int32_t b = blockIdx.y;
-  const int32_t split = blockIdx.z;
-  const int32_t heads = min(16, p.group - g0);
-  const int32_t qh0 = h * p.group + g0;
-
-  int32_t ctx = p.context_lengths[b];
+  w.h = blockIdx.x / head_tiles;
+  const int32_t g0 = (blockIdx.x - w.h * head_tiles) * 16;
+  w.b = blockIdx.y;
+  w.split = blockIdx.z;
+  w.heads = min(16, p.group - g0);
+  w.qh0 = w.h * p.group + g0;
+  int32_t ctx = p.context_lengths[w.b];
   ctx = ctx < 0 ? 0 : (ctx > p.max_tokens ? p.max_tokens : ctx);
-  const int32_t begin = static_cast<int32_t>(min(static_cast<int64_t>(split) * p.split_size, static_cast<int64_t>(ctx)));
-  const int32_t end = ctx - begin < p.split_size ? ctx : begin + p.split_size;
-  if (begin >= end) {
-    if (p.num_splits == 1) {
-      T *out = static_cast<T *>(p.output) + (static_cast<int64_t>(b) * p.query_heads + qh0) * D;
-      for (int i = threadIdx.x; i < heads * D; i += blockDim.x) out[i] = from_float<T>(0.f);
-    }
-    return;
-  }
+  w.begin = static_cast<int32_t>(min(static_cast<int64_t>(w.split) * p.split_size, static_cast<int64_t>(ctx)));
+  w.end = ctx - w.begin < p.split_size ? ctx : w.begin + p.split_size;
+  return w;
+}
 
-  // Queries: lane (head, quad) holds dimensions 64 u + 16 quad .. + 15.
-  bf16x8 q[KU][2][PARTS];
-  const T *query = static_cast<const T *>(p.query) + (static_cast<int64_t>(b) * p.query_heads + qh0 + min(col, heads - 1)) * D;
-#pragma unroll
-  for (int u = 0; u < KU; ++u)
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float x[8];
-      const int32_t d = 64 * u + 16 * quad + 8 * half;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = !GUARD || d < D ? to_float(query[d + j]) : 0.f;
-      split_parts<PARTS>(x, q[u][half]);
-    }
+// A row without tokens is zeros; a partition without them leaves nothing.
+template <typename T>
+__device__ __forceinline__ void finish_empty(const Q8Params &p, const Part &w) {
+  if (p.num_splits != 1) return;
+  T *out = static_cast<T *>(p.output) + (static_cast<int64_t>(w.b) * p.query_heads + w.qh0) * p.head_dim;
+  for (int i = threadIdx.x; i < w.heads * p.head_dim; i += blockDim.x) out[i] = from_float<T>(0.f);
+}
 
-  // A tile is 16 tokens of a page; `per_page` of them in a page.
-  const int32_t per_page = p.block_size >> 4;
-  const int32_t *table = p.block_tables + static_cast<int64_t>(b) * p.table_width;
-  const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * p.block_size * D;
-  const int64_t head_offset = static_cast<int64_t>(h) * p.block_size * D;
-  struct Place {
-    int32_t page, sub;  // page -1: none
-  };
-  auto place_of = [&](int32_t base) {
-    Place at{-1, 0};
-    const int32_t t = base + 16 * quad;
-    if (base < end && t < end) {
-      const int32_t tile = t >> 4;
-      const int32_t logical = per_page == 1 ? tile : tile / per_page;
-      at.page = table[logical];
-      at.sub = per_page == 1 ? 0 : tile - logical * per_page;
-    }
-    return at;
-  };
-  auto load = [&](Block<DMAX> &blk, Place at, int32_t base) {
-    if (base >= end) return;
-    const bool inside = at.page >= 0 && at.page < p.num_blocks;
-    blk.tokens = inside ? min(16, end - (base + 16 * quad)) : 0;
-    const int32_t page = inside ? at.page : 0;  // loaded all the same, and masked
-    const int32_t sub = inside ? at.sub : 0;
-    const int64_t scale_at = static_cast<int64_t>(page) * p.kv_heads + h;
-    blk.k_scale = p.key_scales[scale_at];
-    blk.v_scale = p.value_scales[scale_at];
-    const int from = lane & 12;  // lane (0, col / 4): the tile of this lane's key rows
-    const int32_t k_page = __shfl(page, 4 * from, 64);
-    const int32_t k_sub = __shfl(sub, 4 * from, 64);
-    const uint8_t *key = p.key_cache + k_page * page_bytes + head_offset + (16 * k_sub + (col & 3)) * D + 16 * quad;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int u = 0; u < KU; ++u) {
-        if (!GUARD || 64 * u + 16 * quad < D)
-          blk.k[r][u] = load_stream16<u32x4>(key + 4 * r * D + 64 * u);
-        else
-          blk.k[r][u] = u32x4{0, 0, 0, 0};
-      }
-    const uint8_t *value = p.value_cache + page * page_bytes + head_offset + col * p.block_size + 16 * sub;
-#pragma unroll
-    for (int j = 0; j < DT; ++j)
-      if (!GUARD || 16 * j < D) blk.v[j] = load_stream16<u32x4>(value + 16 * j * p.block_size);
-  };
+// A wavefront's queries and running state.  DMAX: head_dim, or with GUARD any
+// head_dim up to it.
+template <typename T, int DMAX, bool GUARD>
+struct Attention {
+  static constexpr int PARTS = kParts<T>;
+  static constexpr int KU = DMAX / 64;  // 16-byte pieces of a key per lane: 64 dimensions each
+  static constexpr int DT = DMAX / 16;  // tiles of the output
 
+  bf16x8 q[KU][2][PARTS];  // lane (head, quad): dimensions 64 u + 16 quad .. + 15
   float m = kNegInf, l = 0.f;
   f32x4 acc[DT];
-#pragma unroll
-  for (int j = 0; j < DT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto attend = [&](Block<DMAX> &blk, int32_t base) {
-    if (base >= end) return;
+  __device__ __forceinline__ void start(const Q8Params &p, const Part &w, int32_t D) {
+    const int col = threadIdx.x & 15, quad = threadIdx.x >> 4 & 3;
+    const T *query = static_cast<const T *>(p.query) +
+                     (static_cast<int64_t>(w.b) * p.query_heads + w.qh0 + min(col, w.heads - 1)) * D;
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float x[8];
+        const int32_t d = 64 * u + 16 * quad + 8 * half;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = !GUARD || d < D ? to_float(query[d + j]) : 0.f;
+        split_parts<PARTS>(x, q[u][half]);
+        // In registers from here: left to their first use, the wait for them
+        // would stand in the loop over blocks and hold its loads.
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) asm volatile("" : "+v"(q[u][half][i]));
+      }
+#pragma unroll
+    for (int j = 0; j < DT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // 64 tokens: k[r] the key rows of product r, v[j] the values of dimensions
+  // 16 j .. + 15; `tokens` of this lane's tile count, with the tile's scales.
+  __device__ __forceinline__ void block(const u32x4 (&k)[4][KU], u32x4 (&v)[DT], uint32_t k_scale, uint32_t v_scale,
+                                        int32_t tokens, float scale_log2, int32_t D) {
     f32x4 s[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -227,32 +188,31 @@ __global__ void __launch_bounds__(512) paged_decode_q8_kernel(Q8Params p) {
       for (int u = 0; u < KU; ++u)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const bf16x8 a = decode8(blk.k[r][u][2 * half], blk.k[r][u][2 * half + 1], 1.f);
+          const bf16x8 a = decode8(k[r][u][2 * half], k[r][u][2 * half + 1], 1.f);
 #pragma unroll
           for (int i = PARTS - 1; i >= 0; --i) s[r] = mfma(a, q[u][half][i], s[r]);
         }
     }
-    const float unit = scale_of(blk.k_scale) * p.scale_log2;
+    const float unit = scale_of(k_scale) * scale_log2;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[r][i] *= unit;
-    const bool whole = __all(blk.tokens >= 16);
-    if (!whole) {
+    if (!__all(tokens >= 16)) {
       // Tokens behind the end or outside the cache: scores of -inf, values of 0
       // (their codes may be anything, NaN too).
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[r][i] = 4 * r + i < blk.tokens ? s[r][i] : kNegInf;
+        for (int i = 0; i < 4; ++i) s[r][i] = 4 * r + i < tokens ? s[r][i] : kNegInf;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const int left = blk.tokens - 4 * w;
+        const int left = tokens - 4 * w;
         const uint32_t keep = left >= 4 ? ~0u : (left <= 0 ? 0u : (1u << (8 * left)) - 1);
 #pragma unroll
-        for (int j = 0; j < DT; ++j) blk.v[j][w] &= keep;
+        for (int j = 0; j < DT; ++j) v[j][w] &= keep;
       }
-      if (blk.tokens <= 0) blk.v_scale = 127;
+      if (tokens <= 0) v_scale = 127;
     }
     float top = kNegInf;
 #pragma unroll
@@ -271,6 +231,7 @@ __global__ void __launch_bounds__(512) paged_decode_q8_kernel(Q8Params p) {
         for (int i = 0; i < 4; ++i) acc[j][i] *= alpha;
       m = next;
     }
+    const float v_unit = scale_of(v_scale);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       float w[8];
@@ -281,103 +242,335 @@ __global__ void __launch_bounds__(512) paged_decode_q8_kernel(Q8Params p) {
       }
       bf16x8 weights[PARTS];
       split_parts<PARTS>(w, weights);
-      const float v_unit = scale_of(blk.v_scale);
 #pragma unroll
       for (int j = 0; j < DT; ++j) {
-        if (GUARD && 16 * j >= D) break;
-        const bf16x8 a = decode8(blk.v[j][2 * half], blk.v[j][2 * half + 1], v_unit);
+        if (!GUARD || 16 * j < D) {
+          const bf16x8 a = decode8(v[j][2 * half], v[j][2 * half + 1], v_unit);
 #pragma unroll
-        for (int i = PARTS - 1; i >= 0; --i) acc[j] = mfma(a, weights[i], acc[j]);
+          for (int i = PARTS - 1; i >= 0; --i) acc[j] = mfma(a, weights[i], acc[j]);
+        }
+      }
+    }
+  }
+
+  // The wavefronts' states meet in LDS (`merged`: [wavefronts][heads][D + 4], a
+  // row the D numerators, l and m) and leave as output or partials.
+  __device__ __forceinline__ void finish(const Q8Params &p, const Part &w, float *merged, int32_t D) {
+    const int col = threadIdx.x & 15, quad = threadIdx.x >> 4 & 3;
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    l = over_quads(l, [](float x, float y) { return x + y; });
+    const int pitch = D + 4;
+    const int next = w.heads * pitch;
+    float *state = merged + wave * next + col * pitch;
+    float top = m;
+    if (waves > 1) {  // every state to the largest maximum, so that the sums below are plain
+      if (quad == 0 && col < w.heads) state[D + 1] = m;
+      __syncthreads();
+      for (int i = 0; i < waves; ++i) top = fmaxf(top, merged[i * next + min(col, w.heads - 1) * pitch + D + 1]);
+      const float alpha = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
+      l *= l == 0.f ? 1.f : (m == kNegInf ? 1.f : alpha);
+#pragma unroll
+      for (int j = 0; j < DT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] *= alpha;
+    }
+    if (col < w.heads) {
+#pragma unroll
+      for (int j = 0; j < DT; ++j)
+        if (!GUARD || 16 * j < D) *reinterpret_cast<f32x4 *>(state + 16 * j + 4 * quad) = acc[j];
+      if (quad == 0) {
+        state[D] = l;
+        if (p.num_splits != 1 && wave == 0)
+          p.partial_max[(static_cast<int64_t>(w.b) * p.query_heads + w.qh0 + col) * p.num_splits + w.split] = top;
+      }
+    }
+    __syncthreads();
+    const int quads = D / 4;
+    for (int item = threadIdx.x; item < w.heads * quads; item += blockDim.x) {
+      const int head = item / quads;
+      const int d = 4 * (item - head * quads);
+      const float *from = merged + head * pitch;
+      float sum = 0.f;
+      f32x4 num{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < waves; ++i) {
+        sum += from[i * next + D];
+        num += *reinterpret_cast<const f32x4 *>(from + i * next + d);
+      }
+      const int64_t row = static_cast<int64_t>(w.b) * p.query_heads + w.qh0 + head;
+      if (p.num_splits == 1) {
+        T *out = static_cast<T *>(p.output) + row * D + d;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[j] = from_float<T>(sum == 0.f ? 0.f : num[j] / sum);
+      } else {
+        const int64_t slot = row * p.num_splits + w.split;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p.partial_acc[slot * p.partial_stride + d + j] = num[j];
+        if (d == 0) p.partial_sum[slot] = sum;
+      }
+    }
+  }
+};
+
+// Any head_dim: the operands loaded straight to registers, block by block.
+template <typename T, int DMAX>
+__global__ void __launch_bounds__(512) paged_decode_q8_kernel(Q8Params p) {
+  using A = Attention<T, DMAX, true>;
+  extern __shared__ float merged[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15;
+  const int quad = lane >> 4;
+  const int32_t D = p.head_dim;
+  const Part w = part_of(p);
+  if (w.begin >= w.end) return finish_empty<T>(p, w);
+  A state;
+  state.start(p, w, D);
+  // A tile is 16 tokens of a page.
+  const int32_t per_page = p.block_size >> 4;
+  const int32_t *table = p.block_tables + static_cast<int64_t>(w.b) * p.table_width;
+  const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * p.block_size * D;
+  const int64_t head_offset = static_cast<int64_t>(w.h) * p.block_size * D;
+  for (int32_t base = w.begin + 64 * wave; base < w.end; base += blockDim.x) {
+    const int32_t t = base + 16 * quad;
+    int32_t page = -1, sub = 0, tokens = 0;
+    if (t < w.end) {
+      const int32_t tile = t >> 4;
+      const int32_t logical = tile / per_page;
+      page = table[logical];
+      sub = tile - logical * per_page;
+      tokens = min(16, w.end - t);
+    }
+    if (page < 0 || page >= p.num_blocks) page = sub = tokens = 0;  // page 0 is loaded and masked
+    const int64_t scale_at = static_cast<int64_t>(page) * p.kv_heads + w.h;
+    const uint32_t k_scale = p.key_scales[scale_at];
+    const uint32_t v_scale = p.value_scales[scale_at];
+    const int from = 4 * (lane & 12);  // lane (0, col / 4): the tile of this lane's key rows
+    const int32_t k_page = __shfl(page, from, 64);
+    const int32_t k_sub = __shfl(sub, from, 64);
+    const uint8_t *key = p.key_cache + k_page * page_bytes + head_offset + (16 * k_sub + (col & 3)) * D + 16 * quad;
+    u32x4 k[4][A::KU], v[A::DT];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int u = 0; u < A::KU; ++u) {
+        k[r][u] = u32x4{0, 0, 0, 0};
+        if (64 * u + 16 * quad < D) k[r][u] = load_stream16<u32x4>(key + 4 * r * D + 64 * u);
+      }
+    const uint8_t *value = p.value_cache + page * page_bytes + head_offset + col * p.block_size + 16 * sub;
+#pragma unroll
+    for (int j = 0; j < A::DT; ++j) {
+      v[j] = u32x4{0, 0, 0, 0};
+      if (16 * j < D) v[j] = load_stream16<u32x4>(value + 16 * j * p.block_size);
+    }
+    state.block(k, v, k_scale, v_scale, tokens, p.scale_log2, D);
+  }
+  state.finish(p, w, merged, D);
+}
+
+// Tiles whose places and scales are in LDS together.
+constexpr int kPanelTiles = 1024;
+
+// A tile of 16 tokens: its page (-1: none), its place in the page, its scales.
+struct Tile {
+  int32_t page;
+  uint16_t sub;
+  uint8_t k_scale, v_scale;
+};
+
+// head_dim 64 and 128: whole tiles, 1 KB an instruction, by direct-to-LDS loads
+// into a buffer of 64 tokens for each wavefront, refilled as soon as its
+// operands are in registers.  Loaded in the operand layout, four rows from
+// each of four tiles an instruction, the keys held the same kernel to
+// 3.5 TB/s.  (Two and three buffers a wavefront: no case faster.)  The places
+// of the partition's tiles are gathered first, their scales and the queries
+// while the first blocks come in, so that the loop waits for nothing but its
+// own blocks.
+template <typename T, int D>
+__global__ void __launch_bounds__(512) paged_decode_q8_stream_kernel(Q8Params p) {
+  using A = Attention<T, D, false>;
+  constexpr int kTileBytes = 16 * D;
+  constexpr int kStage = 8 * kTileBytes;        // four tiles of keys, four of values
+  constexpr int kPieces = D / 16;               // 16-byte pieces of a key
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = blockDim.x >> 6;
+  const int col = lane & 15;
+  const int quad = lane >> 4;
+  const int32_t per_page = p.block_size >> 4;
+  const int32_t *table = p.block_tables + static_cast<int64_t>(blockIdx.y) * p.table_width;
+  // The page of the partition's tile i, whatever the row's length: its load
+  // does not wait for the length's.
+  const int32_t first_tile = static_cast<int32_t>(
+      min(static_cast<int64_t>(blockIdx.z) * p.split_size, static_cast<int64_t>(p.max_tokens)) >> 4);
+  const int32_t last_tile = (p.max_tokens - 1) >> 4;
+  auto page_of = [&](int32_t i) {
+    const int32_t at = first_tile + i;
+    if (at > last_tile) return -1;
+    return table[per_page == 1 ? at : at / per_page];
+  };
+  const int32_t ahead = page_of(threadIdx.x);
+  const Part w = part_of(p);
+  if (w.begin >= w.end) return finish_empty<T>(p, w);
+  unsigned char *ring = smem + wave * kStage;
+  Tile *tiles = reinterpret_cast<Tile *>(smem + waves * kStage);
+  const uint32_t lds0 = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char *)ring));
+  const uint32_t page_bytes = static_cast<uint32_t>(p.kv_heads) * p.block_size * D;
+  const uint32_t head_offset = static_cast<uint32_t>(w.h) * p.block_size * D;
+
+  // Piece i of token t of tile q is kept at i ^ f(q, t), so that the 16 rows of
+  // an operand read, four tokens of four tiles, lie in different banks.
+  auto swizzle = [](int tile, int token) { return D == 64 ? tile : 2 * tile + (token >> 1 & 1); };
+  uint32_t key_at[4][D / 64], value_at[D / 64];
+#pragma unroll
+  for (int half = 0; half < D / 64; ++half) {
+    const int token = half * (1024 / D) + lane / kPieces;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) key_at[i][half] = token * D + 16 * ((lane % kPieces) ^ swizzle(i, token));
+    value_at[half] = (64 * half + lane) * p.block_size;
+  }
+  // A block's four tiles into the buffer.
+  auto load = [&](const u32x4 (&four)[2]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int32_t page = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(four[i / 2][2 * (i & 1)]));
+      const uint32_t sub = __builtin_amdgcn_readfirstlane(four[i / 2][2 * (i & 1) + 1]) & 0xffffu;
+      // (Scalar arithmetic: the bases below come from scalar instructions.)
+      const uint64_t at = static_cast<uint64_t>(page < 0 ? 0u : static_cast<uint32_t>(page)) * page_bytes + head_offset;
+      const uint8_t *key = p.key_cache + (at + sub * (16 * D));
+      const uint8_t *value = p.value_cache + (at + 16 * sub);
+#pragma unroll
+      for (int half = 0; half < D / 64; ++half) {
+        load_lds16<true>(key, key_at[i][half], __builtin_amdgcn_readfirstlane(lds0 + i * kTileBytes + half * 1024));
+        load_lds16<true>(value, value_at[half],
+                   __builtin_amdgcn_readfirstlane(lds0 + (4 + i) * kTileBytes + half * 1024));
       }
     }
   };
-
-  const int32_t step = 64 * waves;
-  int32_t base = begin + 64 * wave;
-  if constexpr (AHEAD) {
-    Block<DMAX> first, second;
-    Place ahead = place_of(base);
-    load(first, ahead, base);
-    ahead = place_of(base + step);
-    for (; base < end; base += 2 * step) {
-      load(second, ahead, base + step);
-      ahead = place_of(base + 2 * step);
-      attend(first, base);
-      load(first, ahead, base + 2 * step);
-      ahead = place_of(base + 3 * step);
-      attend(second, base + step);
-    }
-  } else {
-    for (; base < end; base += step) {
-      Block<DMAX> blk;
-      load(blk, place_of(base), base);
-      attend(blk, base);
-    }
-  }
-  l = over_quads(l, [](float x, float y) { return x + y; });
-
-  // The wavefronts' states: row (wave, head) holds D numerators, m and l.
-  const int pitch = D + 4;
-  if (col < heads) {
-    float *state = merged + (wave * heads + col) * pitch;
+  auto tiles_of = [&](int32_t first, u32x4 (&four)[2]) {
 #pragma unroll
-    for (int j = 0; j < DT; ++j) {
-      if (GUARD && 16 * j >= D) break;
-      *reinterpret_cast<f32x4 *>(state + 16 * j + 4 * quad) = acc[j];
+    for (int i = 0; i < 2; ++i) four[i] = *reinterpret_cast<const u32x4 *>(tiles + first + 2 * i);
+  };
+
+  A state;
+  auto multiply = [&](int32_t first, int32_t tokens, int32_t next) {
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    u32x4 k[4][A::KU], v[A::DT], four[2];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int tile = col >> 2, token = 4 * r + (col & 3);
+#pragma unroll
+      for (int u = 0; u < A::KU; ++u)
+        k[r][u] = *reinterpret_cast<const u32x4 *>(ring + tile * kTileBytes + token * D +
+                                                   16 * ((4 * u + quad) ^ swizzle(tile, token)));
     }
-    if (quad == 0) {
-      state[D] = m;
-      state[D + 1] = l;
-    }
-  }
-  __syncthreads();
-  for (int item = threadIdx.x; item < heads * D; item += blockDim.x) {
-    const int head = item / D;
-    const int d = item - head * D;
-    const float *from = merged + head * pitch;
-    float top = from[D];
-    for (int w = 1; w < waves; ++w) top = fmaxf(top, from[w * heads * pitch + D]);
-    const float shift = top == kNegInf ? 0.f : top;
-    float sum = 0.f, num = 0.f;
-    for (int w = 0; w < waves; ++w) {
-      const float *one = from + w * heads * pitch;
-      const float weight = __builtin_amdgcn_exp2f(one[D] - shift);
-      sum += weight * one[D + 1];
-      num += weight * one[d];
-    }
-    const int64_t row = static_cast<int64_t>(b) * p.query_heads + qh0 + head;
-    if (p.num_splits == 1) {
-      static_cast<T *>(p.output)[row * D + d] = from_float<T>(sum == 0.f ? 0.f : num / sum);
-    } else {
-      const int64_t slot = row * p.num_splits + split;
-      p.partial_acc[slot * p.partial_stride + d] = num;
-      if (d == 0) {
-        p.partial_max[slot] = top;
-        p.partial_sum[slot] = sum;
+#pragma unroll
+    for (int j = 0; j < A::DT; ++j)
+      v[j] = *reinterpret_cast<const u32x4 *>(ring + (4 + quad) * kTileBytes + (16 * j + col) * 16);
+    tiles_of(next >= 0 ? next : first, four);
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 mine = *reinterpret_cast<const u32x2 *>(tiles + first + quad);
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    if (next >= 0) load(four);
+    const int32_t page = static_cast<int32_t>(mine[0]);
+    const uint32_t scales = mine[1] >> 16;
+    const int32_t left = page >= 0 ? tokens - 16 * quad : 0;
+    state.block(k, v, scales & 255u, scales >> 8, left < 16 ? left : 16, p.scale_log2, D);
+  };
+
+  for (int32_t panel = w.begin; panel < w.end; panel += 16 * kPanelTiles) {
+    const int32_t tokens = min(w.end - panel, 16 * kPanelTiles);
+    const int32_t blocks = (tokens + 63) >> 6;
+    if (panel != w.begin) __syncthreads();  // the last panel's tiles are done with
+    for (int32_t i = threadIdx.x; i < 4 * blocks; i += blockDim.x) {
+      Tile tile{-1, 0, 127, 127};  // behind the end or outside: page 0 is loaded and masked
+      if (16 * i < tokens) {
+        const int32_t at = ((panel - w.begin) >> 4) + i;
+        const int32_t page = at == static_cast<int32_t>(threadIdx.x) ? ahead : page_of(at);
+        if (page >= 0 && page < p.num_blocks) {
+          tile.page = page;
+          tile.sub = static_cast<uint16_t>(per_page == 1 ? 0 : (first_tile + at) % per_page);
+        }
       }
+      tiles[i] = tile;
     }
+    __syncthreads();
+    const int32_t mine = (blocks - wave + waves - 1) / waves;
+    auto first_of = [&](int32_t c) { return 4 * (wave + c * waves); };
+    if (mine > 0) {
+      u32x4 four[2];
+      tiles_of(first_of(0), four);
+      load(four);
+    }
+    for (int32_t i = threadIdx.x; i < 4 * blocks; i += blockDim.x) {
+      const int32_t page = tiles[i].page;
+      if (page < 0) continue;
+      const int64_t scale_at = static_cast<int64_t>(page) * p.kv_heads + w.h;
+      tiles[i].k_scale = p.key_scales[scale_at];
+      tiles[i].v_scale = p.value_scales[scale_at];
+    }
+    if (panel == w.begin) state.start(p, w, D);
+    __syncthreads();
+    for (int32_t c = 0; c < mine; ++c)
+      multiply(first_of(c), tokens - 16 * first_of(c), c + 1 < mine ? first_of(c + 1) : -1);
   }
+  __syncthreads();  // every ring is done with
+  state.finish(p, w, reinterpret_cast<float *>(smem), D);
 }
 
-template <typename T, int DMAX, bool GUARD>
-void launch_attention(const Q8Params &p, int32_t batch, int waves, hipStream_t stream) {
+// Bytes of LDS of one wavefront's state when the workgroup's meet.
+int state_bytes(const Q8Params &p) {
+  return (p.group < 16 ? p.group : 16) * (p.head_dim + 4) * static_cast<int>(sizeof(float));
+}
+
+dim3 attention_grid(const Q8Params &p, int32_t batch) {
+  return dim3(p.kv_heads * ((p.group + 15) / 16), batch, p.num_splits);
+}
+
+template <typename T, int DMAX>
+int32_t launch_any(const Q8Params &p, int32_t batch, int waves, hipStream_t stream) {
   // As many wavefronts as leave their states within 64 KB of LDS: three at
   // least (16 heads of 256 dimensions).
-  const int state = (p.group < 16 ? p.group : 16) * (p.head_dim + 4) * static_cast<int>(sizeof(float));
-  const int fit = 64 * 1024 / state;
+  const int fit = 64 * 1024 / state_bytes(p);
   if (waves > fit) waves = fit;
-  hipLaunchKernelGGL((paged_decode_q8_kernel<T, DMAX, GUARD>),
-                     dim3(p.kv_heads * ((p.group + 15) / 16), batch, p.num_splits), dim3(64 * waves), waves * state,
-                     stream, p);
+  hipLaunchKernelGGL((paged_decode_q8_kernel<T, DMAX>), attention_grid(p, batch), dim3(64 * waves),
+                     waves * state_bytes(p), stream, p);
+  return check_launch("paged_gqa_decode_q8");
+}
+
+template <typename T, int D>
+int32_t launch_stream(const Q8Params &p, int32_t batch, int waves, hipStream_t stream) {
+  auto kernel = paged_decode_q8_stream_kernel<T, D>;
+  const int32_t tokens = p.split_size < p.max_tokens ? p.split_size : p.max_tokens;
+  const int tiles = (tokens + 63) / 64 * 4 < kPanelTiles ? (tokens + 63) / 64 * 4 : kPanelTiles;
+  const int ring = waves * 128 * D + tiles * static_cast<int>(sizeof(Tile));
+  const int states = waves * state_bytes(p);
+  const int lds = ring > states ? ring : states;
+  if (lds > 64 * 1024) {
+    // Raise the kernel's dynamic LDS limit once per device (a failure shows
+    // up as a launch error).
+    constexpr int kMaxDevices = 64;
+    static std::atomic<bool> raised[kMaxDevices];
+    int device = 0;
+    if (hipGetDevice(&device) == hipSuccess && device >= 0 && device < kMaxDevices &&
+        !raised[device].load(std::memory_order_acquire)) {
+      if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              160 * 1024) == hipSuccess)
+        raised[device].store(true, std::memory_order_release);
+    }
+  }
+  hipLaunchKernelGGL(kernel, attention_grid(p, batch), dim3(64 * waves), lds, stream, p);
+  return check_launch("paged_gqa_decode_q8");
 }
 
 template <typename T>
-void launch_dims(const Q8Params &p, int32_t batch, int waves, hipStream_t stream) {
-  if (p.head_dim == 64) return launch_attention<T, 64, false>(p, batch, waves, stream);
-  if (p.head_dim == 128) return launch_attention<T, 128, false>(p, batch, waves, stream);
-  if (p.head_dim < 64) return launch_attention<T, 64, true>(p, batch, waves, stream);
-  if (p.head_dim < 128) return launch_attention<T, 128, true>(p, batch, waves, stream);
-  return launch_attention<T, 256, true>(p, batch, waves, stream);
+int32_t launch_dims(const Q8Params &p, int32_t batch, int waves, hipStream_t stream) {
+  if (p.head_dim == 64) return launch_stream<T, 64>(p, batch, waves, stream);
+  if (p.head_dim == 128) return launch_stream<T, 128>(p, batch, waves, stream);
+  if (p.head_dim < 64) return launch_any<T, 64>(p, batch, waves, stream);
+  if (p.head_dim < 128) return launch_any<T, 128>(p, batch, waves, stream);
+  return launch_any<T, 256>(p, batch, waves, stream);
 }
 
 }  // namespace
@@ -404,6 +597,8 @@ extern "C" int32_t tf_paged_gqa_decode_q8(
     return fail(TF_ERROR_UNSUPPORTED, "block tables of more than 2^30 tokens");
   if (batch > 65535 || num_splits > 65535)
     return fail(TF_ERROR_UNSUPPORTED, "grid too large");
+  if (static_cast<int64_t>(kv_heads) * block_size * head_dim > 1 << 30)
+    return fail(TF_ERROR_UNSUPPORTED, "pages of more than 2^30 codes");
   if (batch == 0) return TF_SUCCESS;
   if (!query || !key_cache || !value_cache || !key_scales || !value_scales || !block_tables || !context_lengths ||
       !output)
@@ -442,14 +637,18 @@ extern "C" int32_t tf_paged_gqa_decode_q8(
                    static_cast<int32_t>(reach < capacity ? reach : capacity),
                    scale * kLog2e};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int blocks = ((split_size < p.max_tokens ? split_size : p.max_tokens) + 63) / 64;
-  const int waves = blocks < 1 ? 1 : (blocks < 8 ? blocks : 8);
-  switch (dtype) {
-    case TF_DTYPE_FLOAT32: launch_dims<float>(p, batch, waves, s); break;
-    case TF_DTYPE_FLOAT16: launch_dims<_Float16>(p, batch, waves, s); break;
-    default: launch_dims<__bf16>(p, batch, waves, s); break;
-  }
-  if (int32_t st = check_launch("paged_gqa_decode_q8")) return st;
+  // Wavefronts of a workgroup: eight while every workgroup has a compute unit to
+  // itself, four where units take several (64 rows of 1088 tokens, 4 kv heads of
+  // 64, 256 workgroups: 10.6 us with eight, 11.1 with four; 72 rows to 2048,
+  // 288: 15.4 and 13.9; sixteen were slower everywhere), none without a block.
+  constexpr int64_t kUnits = 256;
+  const int64_t groups = static_cast<int64_t>(kv_heads) * ((p.group + 15) / 16) * batch * num_splits;
+  const int32_t blocks = ((split_size < p.max_tokens ? split_size : p.max_tokens) + 63) / 64;
+  const int waves = std::min(groups <= kUnits ? 8 : 4, std::max(blocks, 1));
+  const int32_t status = dtype == TF_DTYPE_FLOAT32   ? launch_dims<float>(p, batch, waves, s)
+                         : dtype == TF_DTYPE_FLOAT16 ? launch_dims<_Float16>(p, batch, waves, s)
+                                                     : launch_dims<__bf16>(p, batch, waves, s);
+  if (status) return status;
   if (num_splits == 1) return TF_SUCCESS;
   return tf_paged_gqa_decode_merge(partial_max, partial_sum, partial_accumulator, context_lengths, output,
                                    partial_capacity, partial_row_stride, batch, query_heads, head_dim, split_size,

@@ -224,15 +224,31 @@ def paged_kv_read_token_q8(
     return key_output, value_output
 
 
+# Contexts up to which a row is one partition whatever the batch, tokens of the
+# smallest partition, and tokens from which one is cut to spread ragged rows.
+# On MI355X, graph-timed, the merge launch (2.2 us) included: 8 rows of 1000
+# tokens at 4 kv heads of 64 7.6 us in one pass, 7.1-7.5 in partitions; 1 of
+# 2048 9.6 and 6.9 (16 partitions); 32 of up to 2048 fp32 13.3 and 12.4 (2);
+# 16 of up to 4096 at 8 heads of 128 27.2 and 21.9 (2); 4 of 8k-32k 167 and 35.5
+# (8); 1 of 32k 158 and 18.3 (32).
+ONE_PASS_CONTEXT = 1024
+SMALLEST_PARTITION = 128
+LARGEST_PARTITION = 4096
+COMPUTE_UNITS = 256
+
+
 @functools.lru_cache(maxsize=4096, typed=True)
 def attention_q8_plan(launch_context: int, batch: int, kv_heads: int, slot_limit: int) -> tuple[int, int]:
     """(tokens per partition, partitions per row) of a call, from host-known
-    sizes only: enough partitions for four workgroups per compute unit, of at
-    least 256 tokens, as many as the workspace holds per (row, query head)."""
+    sizes only: about one workgroup per compute unit, more where the partitions
+    would pass LARGEST_PARTITION, as many as the workspace holds per (row, query
+    head); one pass for contexts up to ONE_PASS_CONTEXT."""
 
-    rows_heads = max(batch * kv_heads, 1)
-    want = min(max(1, 1024 // rows_heads), max(1, launch_context // 256), max(slot_limit, 1))
-    size = (-(-launch_context // want) + 63) // 64 * 64
+    want = 1
+    if launch_context > ONE_PASS_CONTEXT:
+        want = max(COMPUTE_UNITS // max(batch * kv_heads, 1), launch_context // LARGEST_PARTITION)
+    want = max(1, min(want, slot_limit))
+    size = max((-(-launch_context // want) + 63) // 64 * 64, SMALLEST_PARTITION)
     return size, -(-launch_context // size)
 
 

@@ -160,6 +160,24 @@ def test_c_abi_calls_without_rows_do_nothing():
     assert _score(library, rows=0, logits=None) == 0
 
 
+def test_attention_plan():
+    """Partitions cover the context in multiples of 64 tokens, as many as the
+    workspace holds; one pass for short contexts and full grids."""
+
+    from tensorforge_amd.kernels.cache_q8 import attention_q8_plan
+
+    for context in (1, 63, 64, 300, 1024, 1025, 2048, 5000, 32768, 1 << 20):
+        for batch in (0, 1, 3, 64, 500):
+            for slots in (0, 1, 2, 7, 64, 1 << 20):
+                size, splits = attention_q8_plan(context, batch, 4, slots)
+                assert size % 64 == 0 and splits * size >= context > (splits - 1) * size
+                assert splits <= max(slots, 1)
+    assert attention_q8_plan(1024, 1, 4, 100)[1] == 1
+    assert attention_q8_plan(2048, 64, 4, 100)[1] == 1
+    assert attention_q8_plan(32768, 4, 8, 100) == (4096, 8)
+    assert attention_q8_plan(2048, 1, 4, 100) == (128, 16)
+
+
 def test_quantize_mxfp4_rounds_to_the_nearest_value():
     generator = torch.Generator().manual_seed(3)
     weight = torch.randn(7, 96, generator=generator) * torch.exp(2 * torch.randn(7, 1, generator=generator))
