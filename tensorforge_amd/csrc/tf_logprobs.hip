@@ -8,20 +8,23 @@
 // counted, not summed: where it stands alone log S = log1p of the rest, so a
 // sharp row keeps its small numbers.
 //
-// One workgroup per row, which it reads once: up to NV 16-byte vectors a thread
-// stay in registers for every later look (longer rows are read again behind
-// those).  The alternatives are ordered by value, equal values by index, a NaN
+// One workgroup per row, which it reads once: up to 16 vectors of 16 bytes a
+// thread stay in registers for every later look (longer rows are read again
+// behind those).  The alternatives are ordered by value, equal values by index, a NaN
 // above every number (as in tf_argmax_rows):
 //
-//  * the threads' maxima in 64 groups; the k-th largest group's is a bound t
-//    that at least k elements reach and few pass (of 32,000 normal logits and
-//    k = 20 about 25);
-//  * elements above t go to a list in LDS, in any order; where they are fewer
-//    than k, elements equal to t follow in the order of their index;
+//  * the threads' maxima in 64 groups, one a lane: the k-th largest group's is a
+//    bound t that at least k elements reach and few pass (of 32,000 normal
+//    logits and k = 20 about 25);
+//  * the elements that reach t go to a list in LDS, in any order;
 //  * each of the list counts those ahead of it: its place.
 //
-// Where the list overflows (the largest elements share few groups), t is
-// raised to the k-th largest element itself, found bit by bit.
+// Where the list overflows (ties, or a mask that leaves few groups) it takes the
+// elements above t only, or, if they are still too many, above the k-th
+// largest element, found bit by bit; then elements equal to t follow in the
+// order of their index.
+#include <type_traits>
+
 #include "tf_common.hpp"
 
 namespace tf {
@@ -43,68 +46,90 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-template <typename T, int NV, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+// Combine over the 64 lanes by lane moves of the vector unit; every lane gets
+// the result.
+template <typename V, typename F>
+__device__ __forceinline__ V over_wave(V v, F combine) {
+  static_assert(sizeof(V) == 4, "32-bit values");
+  auto moved = [&](auto ctrl) {
+    const int bits = __builtin_bit_cast(int, v);
+    const int other = __builtin_amdgcn_update_dpp(bits, bits, decltype(ctrl)::value, 0xf, 0xf, false);
+    return __builtin_bit_cast(V, other);
+  };
+  v = combine(v, moved(std::integral_constant<int, 0xb1>{}));   // lane ^ 1
+  v = combine(v, moved(std::integral_constant<int, 0x4e>{}));   // lane ^ 2
+  v = combine(v, moved(std::integral_constant<int, 0x141>{}));  // the other quad of eight
+  v = combine(v, moved(std::integral_constant<int, 0x140>{}));  // the other eight of sixteen
+  uint32_t bits = __builtin_bit_cast(uint32_t, v);
+  const auto rows = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+  const uint32_t even = rows[0], odd = rows[1];
+  v = combine(__builtin_bit_cast(V, even), __builtin_bit_cast(V, odd));
+  bits = __builtin_bit_cast(uint32_t, v);
+  const auto halves = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+  const uint32_t low = halves[0], high = halves[1];
+  return combine(__builtin_bit_cast(V, low), __builtin_bit_cast(V, high));
+}
+
+// NV vectors of VEC elements a thread in registers; NV = 0 (and VEC = 1, rows
+// that 16-byte loads cannot take): none, every look reads the row.
+template <typename T, int VEC, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(NV <= 4 ? 8 : 4)))
 token_logprobs_kernel(const T *__restrict__ logits, int64_t row_stride, int32_t columns,
                       const int64_t *__restrict__ tokens, float *__restrict__ logprobs, float *__restrict__ entropy,
                       float *__restrict__ top_logprobs, int64_t *__restrict__ top_tokens, int32_t top_k) {
-  constexpr int VEC = 16 / sizeof(T);
-  constexpr int kWaves = THREADS / 64;
-  constexpr int kPass = THREADS * NV;             // vectors of a pass
-  constexpr int kGroupLanes = THREADS / kGroups;  // 4 or 16
-  struct alignas(16) Vec {
+  struct alignas(sizeof(T) * VEC) Vec {
     T v[VEC];
   };
+  constexpr int kWaves = THREADS / 64;
   __shared__ uint32_t group_keys[kGroups];
-  __shared__ float wave_sums[kWaves], wave_weighted[kWaves];
+  __shared__ float wave_tops[kWaves], wave_sums[kWaves], wave_weighted[kWaves];
   __shared__ int32_t wave_ones[kWaves], counts[2][kWaves];
   __shared__ uint32_t bound_key;
   __shared__ int32_t listed;
   __shared__ uint32_t list_key[kList];
-  __shared__ int32_t list_index[kList];
+  __shared__ int32_t list_index[kList], places[kList];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t r = blockIdx.x;
   const T *row = logits + r * row_stride;
-  // Vector i holds columns VEC i - skew .. + VEC - 1: aligned whatever the row's
-  // start is.  Those the row does not fill are loaded element by element.
-  const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
-  const int32_t vectors = (columns + skew + VEC - 1) / VEC;
-  const T absent = from_float<T>(-__builtin_inff());
-  auto load = [&](int32_t i) {
-    Vec v;
-    const int32_t c = i * VEC - skew;
-    if (c >= 0 && c + VEC <= columns) {
-      v = *reinterpret_cast<const Vec *>(row + c);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v.v[e] = c + e >= 0 && c + e < columns ? row[c + e] : absent;
-    }
-    return v;
-  };
-  Vec held[NV];
+  const Vec *vrow = reinterpret_cast<const Vec *>(row);
+  const int32_t vectors = columns / VEC;
+  // Columns behind the last whole vector, one a thread.
+  const int32_t last = vectors * VEC + tid;
+  const bool has_last = last < columns;
+  Vec held[NV > 0 ? NV : 1];
 #pragma unroll
   for (int u = 0; u < NV; ++u)
-    if (u * THREADS + tid < vectors) held[u] = load(u * THREADS + tid);
-  // f(value, column, whether it is one) for this thread's elements, in the
-  // order of their column.
-  auto visit = [&](auto f) {
+    if (u * THREADS + tid < vectors) held[u] = vrow[u * THREADS + tid];
+  const T last_value = has_last ? row[last] : from_float<T>(0.f);
+  // f(vector, its number) for this thread's, in order.  The packed vectors are
+  // made new to the compiler each time, which otherwise keeps every element
+  // unpacked in a register of its own.
+  auto each_vector = [&](auto f) __attribute__((always_inline)) {
+    if constexpr (NV > 0) {
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      const int32_t i = u * THREADS + tid;
-      if (i >= vectors) continue;
+      for (int u = 0; u < NV; ++u) {
+        u32x4 bits = __builtin_bit_cast(u32x4, held[u]);
+        asm volatile("" : "+v"(bits));
+        held[u] = __builtin_bit_cast(Vec, bits);
+      }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f(to_float(held[u].v[e]), i * VEC - skew + e);
+      for (int u = 0; u < NV; ++u)
+        if (u * THREADS + tid < vectors) f(held[u], u * THREADS + tid);
     }
-    for (int32_t i = kPass + tid; i < vectors; i += THREADS) {
-      const Vec v = load(i);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) f(to_float(v.v[e]), i * VEC - skew + e);
-    }
+    for (int32_t i = NV * THREADS + tid; i < vectors; i += THREADS) f(vrow[i], i);
   };
-  auto inside = [&](int32_t c) { return static_cast<uint32_t>(c) < static_cast<uint32_t>(columns); };
+  // f(value, column) for every element of this thread's.
+  auto visit = [&](auto f) __attribute__((always_inline)) {
+    each_vector([&](const Vec &v, int32_t i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f(to_float(v.v[e]), i * VEC + e);
+    });
+    if (has_last) f(to_float(last_value), last);
+  };
 
+  if (tid < kGroups) group_keys[tid] = 0;
   int64_t token = -1;
   float given = __builtin_nanf("");
   if (tid == 0) {
@@ -113,70 +138,55 @@ token_logprobs_kernel(const T *__restrict__ logits, int64_t row_stride, int32_t 
     if (token >= 0 && token < columns) given = to_float(row[token]);
   }
 
-  // The largest value (absent ones are -inf), as a key with NaN on top.
   float own = -__builtin_inff();
-  bool nan = false;
-  visit([&](float x, int32_t) {
-    own = fmaxf(own, x);
-    nan |= x != x;
-  });
-  const bool any = tid < vectors;
-  const uint32_t own_key = !any ? 0u : nan ? 0xffffffffu : order_key(own);
-  uint32_t key = own_key;
-  float top = own;
-#pragma unroll
-  for (int offset = 1; offset < kGroupLanes; offset <<= 1)
-    key = max(key, static_cast<uint32_t>(__shfl_xor(static_cast<int>(key), offset, 64)));
-  if (lane % kGroupLanes == 0) group_keys[tid / kGroupLanes] = key;
-  top = wave_max(top);
-  if (lane == 0) wave_sums[wave] = top;
+  visit([&](float x, int32_t) { own = fmaxf(own, x); });
+  const auto larger = [](float a, float b) { return fmaxf(a, b); };
+  const float wave_top = over_wave(own, larger);
+  if (lane == 0) wave_tops[wave] = wave_top;
   __syncthreads();
-  float m = wave_sums[0];
+  float m = wave_tops[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, wave_sums[w]);
-  if (top_k > 0) {
-    // The groups with fewer than top_k ahead of them, equal ones in order; each
-    // wavefront looks at its own.
-    const uint32_t mine = group_keys[lane];
-    constexpr int kOwn = 64 / kGroupLanes;
-#pragma unroll
-    for (int g = 0; g < kOwn; ++g) {
-      const int at = wave * kOwn + g;
-      const uint32_t one = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), at));
-      const unsigned long long above = __ballot(mine > one), same = __ballot(mine == one);
-      const int ahead = __popcll(above) + __popcll(same & ((1ull << at) - 1));
-      if (ahead == top_k - 1 && lane == 0) bound_key = one;
-    }
-  }
+  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, wave_tops[w]);
 
+  // In units of log2: t = (x - m) log2 e, e = 2^t, which is 0 from t = -150 on:
+  // t is held above -200 in t e, so that x = -inf adds 0 to it.
+  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
   float sum = 0.f, weighted = 0.f;
   int32_t ones = 0;
   if (own == m) {
-    visit([&](float x, int32_t c) {
-      const float d = x - m;
-      const float e = __expf(d);
-      ones += d == 0.f && inside(c);
-      sum += d == 0.f ? 0.f : e;
-      weighted += e == 0.f ? 0.f : d * e;
+    visit([&](float x, int32_t) {
+      const float t = (x - m) * kLog2e;
+      const float e = __builtin_amdgcn_exp2f(t);
+      ones += t == 0.f;
+      sum += t == 0.f ? 0.f : e;
+      weighted = __builtin_fmaf(fmaxf(t, -200.f), e, weighted);
     });
   } else {
     visit([&](float x, int32_t) {
-      const float d = x - m;
-      const float e = __expf(d);
+      const float t = (x - m) * kLog2e;
+      const float e = __builtin_amdgcn_exp2f(t);
       sum += e;
-      weighted += e == 0.f ? 0.f : d * e;
+      weighted = __builtin_fmaf(fmaxf(t, -200.f), e, weighted);
     });
   }
-  sum = wave_sum(sum);
-  weighted = wave_sum(weighted);
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) ones += __shfl_xor(ones, offset, 64);
-  __syncthreads();  // the maxima have been read
+  // The thread's largest element as a key, 0 without any.  A sum that is NaN
+  // came from one, or from x - m of infinities.
+  bool nan = sum != sum;
+  if (__builtin_isinf(m)) {
+    nan = false;
+    visit([&](float x, int32_t) { nan |= x != x; });
+  }
+  const uint32_t own_key = tid >= vectors && !has_last ? 0u : nan ? 0xffffffffu : order_key(own);
+  const auto add = [](auto a, auto b) { return a + b; };
+  sum = over_wave(sum, add);
+  weighted = over_wave(weighted, add);
+  if (__any(ones != 0)) ones = over_wave(ones, add);
   if (lane == 0) {
     wave_sums[wave] = sum;
     wave_weighted[wave] = weighted;
     wave_ones[wave] = ones;
   }
+  if (top_k > 0) atomicMax(&group_keys[lane], own_key);
   __syncthreads();
   sum = weighted = 0.f;
   ones = 0;
@@ -186,70 +196,100 @@ token_logprobs_kernel(const T *__restrict__ logits, int64_t row_stride, int32_t 
     weighted += wave_weighted[w];
     ones += wave_ones[w];
   }
-  const float log_sum = ones == 1 ? log1pf(sum) : logf(static_cast<float>(ones) + sum);
+  const float all = static_cast<float>(ones) + sum;
+  const float log_sum = ones == 1 ? log1pf(sum) : logf(all);
   if (tid == 0) {
     logprobs[r] = (given - m) - log_sum;
-    entropy[r] = log_sum - weighted / (static_cast<float>(ones) + sum);
+    entropy[r] = log_sum - weighted * kLn2 / all;
   }
   if (top_k == 0) return;
 
-  uint32_t bound = bound_key;
-  auto list_above = [&] {
-    if (own_key > bound)
-      visit([&](float x, int32_t c) {
-        if (!inside(c)) return;
-        const uint32_t k = order_key(x);
-        if (k <= bound) return;
-        const int32_t at = atomicAdd(&listed, 1);
-        if (at < kList) {
-          list_key[at] = k;
-          list_index[at] = c;
-        }
-      });
-    __syncthreads();
-    return listed;
-  };
-  int32_t above = list_above();
-  if (above > kList) {
-    // The k-th largest key, from its highest bit down.
-    uint32_t found = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t trial = found | 1u << bit;
-      int32_t mine = 0;
-      if (own_key >= trial) visit([&](float x, int32_t c) { mine += inside(c) && order_key(x) >= trial; });
+  // The top_k-th of the groups, equal ones in order; each wavefront looks at its
+  // share of them.
+  {
+    const uint32_t mine = group_keys[lane];
+    constexpr int kOwn = kGroups / kWaves;
 #pragma unroll
-      for (int offset = 32; offset > 0; offset >>= 1) mine += __shfl_xor(mine, offset, 64);
-      if (lane == 0) counts[bit & 1][wave] = mine;
-      __syncthreads();
-      int32_t all = 0;
-      for (int w = 0; w < kWaves; ++w) all += counts[bit & 1][w];
-      if (all >= top_k) found = trial;
+    for (int g = 0; g < kOwn; ++g) {
+      const int at = wave * kOwn + g;
+      const uint32_t one = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), at));
+      const unsigned long long above = __ballot(mine > one), same = __ballot(mine == one);
+      const int ahead = __popcll(above) + __popcll(same & ((1ull << at) - 1));
+      if (ahead == top_k - 1 && lane == 0) bound_key = one;
     }
-    bound = found;
+  }
+  __syncthreads();
+  uint32_t bound = bound_key;
+  // The elements whose key is at least `least` into the list; where they overflow
+  // it, those above the bound, and then above the top_k-th largest.
+  uint32_t least = bound;
+  int32_t above;
+  for (int attempt = 0;; ++attempt) {
+    const float value = key_value(least);
+    auto list = [&](float x, int32_t c) __attribute__((always_inline)) {
+      const uint32_t k = order_key(x);
+      if (k < least) return;
+      const int32_t at = atomicAdd(&listed, 1);
+      if (at < kList) {
+        list_key[at] = k;
+        list_index[at] = c;
+      }
+    };
+    if (own_key >= least) {
+      each_vector([&](const Vec &v, int32_t i) __attribute__((always_inline)) {
+        float most = to_float(v.v[0]);
+#pragma unroll
+        for (int e = 1; e < VEC; ++e) most = fmaxf(most, to_float(v.v[e]));
+        if (most < value && own_key != 0xffffffffu) return;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) list(to_float(v.v[e]), i * VEC + e);
+      });
+      if (has_last) list(to_float(last_value), last);
+    }
+    __syncthreads();
+    above = listed;
+    if (above <= kList) break;
+    if (attempt == 1) {
+      // The top_k-th largest key, from its highest bit down.
+      uint32_t found = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t trial = found | 1u << bit;
+        int32_t mine = 0;
+        if (own_key >= trial) visit([&](float x, int32_t) { mine += order_key(x) >= trial; });
+        mine = over_wave(mine, add);
+        if (lane == 0) counts[bit & 1][wave] = mine;
+        __syncthreads();
+        int32_t reach = 0;
+        for (int w = 0; w < kWaves; ++w) reach += counts[bit & 1][w];
+        if (reach >= top_k) found = trial;
+      }
+      bound = found;
+    }
+    if (bound == 0xffffffffu) {  // NaN: nothing is above it
+      least = 0;
+      above = 0;
+      break;
+    }
+    least = bound + 1;
     __syncthreads();
     if (tid == 0) listed = 0;
     __syncthreads();
-    above = list_above();
   }
-  // Elements equal to the bound, by index, up to top_k.
-  if (above < top_k) {
+  if (least != bound && above < top_k) {
+    // Elements equal to the bound, by index, up to top_k: whole vectors, a round
+    // of the workgroup at a time, then the columns behind them.
     int32_t have = above;
-    for (int32_t first = 0; first < vectors && have < top_k; first += THREADS) {
+    for (int32_t first = 0, round = 0; have < top_k && first < vectors + THREADS; first += THREADS, ++round) {
       const int32_t i = first + tid;
       uint32_t hits = 0;
-      if (i < vectors && own_key >= bound) {
-        Vec v;
-        bool kept = false;
+      int32_t column = i * VEC;
+      if (first >= vectors) {
+        column = last;
+        hits = has_last && order_key(to_float(last_value)) == bound;
+      } else if (i < vectors && own_key >= bound) {
+        Vec v = vrow[i];
 #pragma unroll
-        for (int u = 0; u < NV; ++u)
-          if (first == u * THREADS) {
-            v = held[u];
-            kept = true;
-          }
-        if (!kept) v = load(i);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          hits |= (inside(i * VEC - skew + e) && order_key(to_float(v.v[e])) == bound ? 1u : 0u) << e;
+        for (int e = 0; e < VEC; ++e) hits |= (order_key(to_float(v.v[e])) == bound ? 1u : 0u) << e;
       }
       const int32_t mine = __popc(hits);
       int32_t before = 0, wave_total = 0;  // equal elements of earlier lanes, and of the wavefront
@@ -259,19 +299,18 @@ token_logprobs_kernel(const T *__restrict__ logits, int64_t row_stride, int32_t 
         before += e * __popcll(with & ((1ull << lane) - 1));
         wave_total += e * __popcll(with);
       }
-      const int buffer = first / THREADS & 1;
-      if (lane == 0) counts[buffer][wave] = wave_total;
+      if (lane == 0) counts[round & 1][wave] = wave_total;
       __syncthreads();
       int32_t at = have + before;
       for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) at += counts[buffer][w];
-        have += counts[buffer][w];
+        if (w < wave) at += counts[round & 1][w];
+        have += counts[round & 1][w];
       }
       for (int e = 0; e < VEC; ++e)
         if (hits >> e & 1) {
           if (at < top_k) {
             list_key[at] = bound;
-            list_index[at] = i * VEC - skew + e;
+            list_index[at] = column + e;
           }
           ++at;
         }
@@ -279,20 +318,29 @@ token_logprobs_kernel(const T *__restrict__ logits, int64_t row_stride, int32_t 
     __syncthreads();
     above = top_k;
   }
-  for (int32_t c = tid; c < above; c += THREADS) {
+  // Lanes take the list's elements, wavefronts the ones compared with.
+  for (int32_t c = tid; c < above; c += THREADS) places[c] = 0;
+  __syncthreads();
+  for (int32_t c = lane; c < above; c += 64) {
     const uint32_t k = list_key[c];
     const int32_t index = list_index[c];
     int32_t ahead = 0;
-    for (int32_t o = 0; o < above; ++o) ahead += list_key[o] > k || (list_key[o] == k && list_index[o] < index);
-    if (ahead < top_k) {
-      top_tokens[r * top_k + ahead] = index;
-      top_logprobs[r * top_k + ahead] = (key_value(k) - m) - log_sum;
-    }
+    for (int32_t o = wave; o < above; o += kWaves)
+      ahead += list_key[o] > k || (list_key[o] == k && list_index[o] < index);
+    if (ahead) atomicAdd(&places[c], ahead);
+  }
+  __syncthreads();
+  for (int32_t c = tid; c < above; c += THREADS) {
+    const int32_t place = places[c];
+    if (place >= top_k) continue;
+    top_tokens[r * top_k + place] = list_index[c];
+    top_logprobs[r * top_k + place] = (key_value(list_key[c]) - m) - log_sum;
   }
 }
 
 template <typename T>
 struct Rows {
+  static constexpr int VEC = 16 / sizeof(T);
   const T *logits;
   int64_t row_stride;
   int32_t rows, columns;
@@ -301,29 +349,22 @@ struct Rows {
   int64_t *top_tokens;
   int32_t top_k;
 
-  template <int NV, int THREADS>
+  template <int V, int NV, int THREADS>
   void launch(hipStream_t stream) const {
-    hipLaunchKernelGGL((token_logprobs_kernel<T, NV, THREADS>), dim3(static_cast<unsigned>(rows)), dim3(THREADS), 0,
+    hipLaunchKernelGGL((token_logprobs_kernel<T, V, NV, THREADS>), dim3(static_cast<unsigned>(rows)), dim3(THREADS), 0,
                        stream, logits, row_stride, columns, tokens, logprobs, entropy, top_logprobs, top_tokens, top_k);
   }
+  // With the fewest of 1, 2, 4, 8, 16 vectors a thread that hold the row.
   template <int THREADS>
-  void launch(int nv, hipStream_t stream) const {
-    switch (nv) {
-      case 1: return launch<1, THREADS>(stream);
-      case 2: return launch<2, THREADS>(stream);
-      case 4: return launch<4, THREADS>(stream);
-      case 8: return launch<8, THREADS>(stream);
-      default: return launch<16, THREADS>(stream);
-    }
+  void launch(hipStream_t stream) const {
+    const int64_t each = (columns / VEC + THREADS - 1) / THREADS;
+    if (each <= 1) return launch<VEC, 1, THREADS>(stream);
+    if (each <= 2) return launch<VEC, 2, THREADS>(stream);
+    if (each <= 4) return launch<VEC, 4, THREADS>(stream);
+    if (each <= 8) return launch<VEC, 8, THREADS>(stream);
+    return launch<VEC, 16, THREADS>(stream);
   }
 };
-
-// Vectors a thread holds: the fewest of 1, 2, 4, 8, 16 for the row.
-inline int held_vectors(int64_t vectors, int threads) {
-  int nv = 1;
-  while (nv < 16 && static_cast<int64_t>(nv) * threads < vectors) nv *= 2;
-  return nv;
-}
 
 template <typename T>
 void launch_logprobs(const void *logits, int64_t row_stride, int32_t rows, int32_t columns, const int64_t *tokens,
@@ -331,11 +372,13 @@ void launch_logprobs(const void *logits, int64_t row_stride, int32_t rows, int32
                      hipStream_t stream) {
   const Rows<T> all{static_cast<const T *>(logits), row_stride, rows, columns, tokens, logprobs, entropy,
                     top_logprobs, top_tokens, top_k};
-  const int64_t vectors = static_cast<int64_t>(columns) * sizeof(T) / 16 + 2;
-  if (vectors <= 1024)
-    all.template launch<256>(held_vectors(vectors, 256), stream);
+  const bool whole = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && row_stride % Rows<T>::VEC == 0;
+  if (!whole)
+    all.template launch<1, 0, 1024>(stream);
+  else if (columns / Rows<T>::VEC <= 1024)
+    all.template launch<256>(stream);
   else
-    all.template launch<1024>(held_vectors(vectors, 1024), stream);
+    all.template launch<1024>(stream);
 }
 
 }  // namespace
