@@ -37,17 +37,37 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
   return v;
 }
 
-__device__ __forceinline__ float decode(uint8_t code) { return __builtin_amdgcn_cvt_f32_fp8(code, 0); }
-
-// e4m3 of x, |x| <= 448 or NaN, round to nearest even.
-__device__ __forceinline__ uint8_t encode(float x) {
-  return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false));
+// e4m3 of four values, |x| <= 448 or NaN, round to nearest even, in a word.
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  const int low = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, low, true));
 }
 
-// e4m3 of x * 2^-exponent; infinities become NaN (e4m3 has no infinity).
-__device__ __forceinline__ uint8_t encode_scaled(float x, int32_t exponent) {
+// x * 2^-exponent; infinities become NaN (e4m3 has no infinity).
+__device__ __forceinline__ float scaled(float x, int32_t exponent) {
   const bool finite = (__builtin_bit_cast(uint32_t, x) & 0x7fffffffu) < 0x7f800000u;
-  return encode(finite ? ldexpf(x, -exponent) : __builtin_nanf(""));
+  return finite ? ldexpf(x, -exponent) : __builtin_nanf("");
+}
+
+// The codes of four values under a scale of 2^exponent.
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, int32_t exponent) {
+  return pack4(scaled(a, exponent), scaled(b, exponent), scaled(c, exponent), scaled(d, exponent));
+}
+
+// Four codes times 2^exponent.
+__device__ __forceinline__ void decode4(uint32_t codes, int32_t exponent, float *x) {
+  const int word = static_cast<int>(codes);
+  x[0] = ldexpf(__builtin_amdgcn_cvt_f32_fp8(word, 0), exponent);
+  x[1] = ldexpf(__builtin_amdgcn_cvt_f32_fp8(word, 1), exponent);
+  x[2] = ldexpf(__builtin_amdgcn_cvt_f32_fp8(word, 2), exponent);
+  x[3] = ldexpf(__builtin_amdgcn_cvt_f32_fp8(word, 3), exponent);
+}
+
+// Four codes rounded to a scale 2^-exponent times theirs (exponent < 0).
+__device__ __forceinline__ uint32_t rescale4(uint32_t codes, int32_t exponent) {
+  float x[4];
+  decode4(codes, exponent, x);
+  return pack4(x[0], x[1], x[2], x[3]);
 }
 
 }  // namespace tf
