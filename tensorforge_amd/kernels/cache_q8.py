@@ -41,7 +41,7 @@ class PagedKVCacheQ8:
     value_scales: Tensor
 
     def __post_init__(self) -> None:
-        key, value = self.key, self.value
+        key, value, key_scales, value_scales = self.key, self.value, self.key_scales, self.value_scales
         if key.ndim != 4 or value.ndim != 4:
             raise ValueError("cache codes must be [blocks, kv_heads, block_size, head_dim] keys and "
                              "[blocks, kv_heads, head_dim, block_size] values")
@@ -56,15 +56,15 @@ class PagedKVCacheQ8:
             raise ValueError("the 8-bit cache takes head dimensions that are multiples of 16 up to 256")
         if block_size % 16 or not 0 < block_size <= MAX_BLOCK_SIZE:
             raise ValueError("the 8-bit cache takes pages of a multiple of 16 tokens up to 1024")
-        for scales in (self.key_scales, self.value_scales):
-            if scales.shape != (blocks, kv_heads):
-                raise ValueError("scales must be [blocks, kv_heads]")
-            if scales.dtype != torch.float8_e8m0fnu:
-                raise TypeError("scales must use torch.float8_e8m0fnu")
-        tensors = (key, value, self.key_scales, self.value_scales)
-        if any(tensor.device != key.device for tensor in tensors):
+        if key_scales.shape != (blocks, kv_heads) or value_scales.shape != (blocks, kv_heads):
+            raise ValueError("scales must be [blocks, kv_heads]")
+        if key_scales.dtype != torch.float8_e8m0fnu or value_scales.dtype != torch.float8_e8m0fnu:
+            raise TypeError("scales must use torch.float8_e8m0fnu")
+        device = key.device
+        if value.device != device or key_scales.device != device or value_scales.device != device:
             raise ValueError("cache tensors must share one device")
-        if any(not tensor.is_contiguous() for tensor in tensors):
+        if not (key.is_contiguous() and value.is_contiguous() and key_scales.is_contiguous()
+                and value_scales.is_contiguous()):
             raise ValueError("cache tensors must be contiguous")
         if key.data_ptr() % 16 or value.data_ptr() % 16:
             raise ValueError("cache codes must be 16-byte aligned")
@@ -107,20 +107,20 @@ def _require_library() -> None:
         )
 
 
-def _check_slots(rows: int, device: torch.device, **vectors: Tensor) -> None:
-    for name, tensor in vectors.items():
-        if tensor.shape != (rows,) or tensor.dtype != torch.int32:
-            raise ValueError(f"{name} must be int32 with one value per row")
-        if tensor.device != device or not tensor.is_contiguous():
-            raise ValueError(f"{name} must be contiguous on the cache's device")
+def _check_slots(name: str, tensor: Tensor, rows: int, device: torch.device) -> None:
+    if tensor.dtype != torch.int32 or tensor.shape != (rows,):
+        raise ValueError(f"{name} must be int32 with one value per row")
+    if tensor.device != device or not tensor.is_contiguous():
+        raise ValueError(f"{name} must be contiguous on the cache's device")
 
 
-def _check_rows(name: str, tensor: Tensor, cache: PagedKVCacheQ8, rows: int, dtype: torch.dtype) -> None:
-    if tensor.shape != (rows, cache.kv_heads, cache.head_dim):
+def _check_rows(name: str, tensor: Tensor, shape: tuple[int, int, int], dtype: torch.dtype,
+                device: torch.device) -> None:
+    if tensor.shape != shape:
         raise ValueError(f"{name} must be [rows, kv_heads, head_dim] of the cache's heads")
     if tensor.dtype != dtype:
         raise ValueError("keys and values must share dtype")
-    if tensor.device != cache.key.device or not tensor.is_contiguous():
+    if tensor.device != device or not tensor.is_contiguous():
         raise ValueError(f"{name} must be contiguous on the cache's device")
 
 
@@ -153,20 +153,23 @@ def paged_kv_write_token_q8(
     if device.index != _native.current_device():
         with torch.cuda.device(device):
             return paged_kv_write_token_q8(keys, values, cache, physical_blocks, block_offsets, active_mask)
-    if keys.dtype not in _native.DTYPE_CODES:
-        raise TypeError(f"unsupported dtype: {keys.dtype}")
+    dtype = keys.dtype
+    if dtype not in _native.DTYPE_CODES:
+        raise TypeError(f"unsupported dtype: {dtype}")
     rows = keys.shape[0] if keys.ndim else 0
-    _check_rows("keys", keys, cache, rows, keys.dtype)
-    _check_rows("values", values, cache, rows, keys.dtype)
-    _check_slots(rows, device, physical_blocks=physical_blocks, block_offsets=block_offsets,
-                 active_mask=active_mask)
     num_blocks, kv_heads, block_size, head_dim = cache.key.shape
+    shape = (rows, kv_heads, head_dim)
+    _check_rows("keys", keys, shape, dtype, device)
+    _check_rows("values", values, shape, dtype, device)
+    _check_slots("physical_blocks", physical_blocks, rows, device)
+    _check_slots("block_offsets", block_offsets, rows, device)
+    _check_slots("active_mask", active_mask, rows, device)
     _native.check(
         _native.launch().tf_paged_kv_write_token_q8(
             keys.data_ptr(), values.data_ptr(), cache.key.data_ptr(), cache.value.data_ptr(),
             cache.key_scales.data_ptr(), cache.value_scales.data_ptr(), physical_blocks.data_ptr(),
             block_offsets.data_ptr(), active_mask.data_ptr(), rows, kv_heads, head_dim, num_blocks, block_size,
-            _native.dtype_code(keys.dtype), _native.current_stream(device),
+            _native.dtype_code(dtype), _native.current_stream(device),
         ),
         "paged_kv_write_token_q8",
     )
@@ -205,13 +208,17 @@ def paged_kv_read_token_q8(
         raise ValueError("physical_blocks must be int32 with one value per row")
     rows = physical_blocks.shape[0]
     num_blocks, kv_heads, block_size, head_dim = cache.key.shape
+    shape = (rows, kv_heads, head_dim)
+    _check_slots("physical_blocks", physical_blocks, rows, device)
+    _check_slots("block_offsets", block_offsets, rows, device)
     if key_output is None:
-        key_output = torch.empty((rows, kv_heads, head_dim), dtype=dtype, device=device)
+        key_output = torch.empty(shape, dtype=dtype, device=device)
+    else:
+        _check_rows("key_output", key_output, shape, dtype, device)
     if value_output is None:
-        value_output = torch.empty((rows, kv_heads, head_dim), dtype=dtype, device=device)
-    _check_rows("key_output", key_output, cache, rows, dtype)
-    _check_rows("value_output", value_output, cache, rows, dtype)
-    _check_slots(rows, device, physical_blocks=physical_blocks, block_offsets=block_offsets)
+        value_output = torch.empty(shape, dtype=dtype, device=device)
+    else:
+        _check_rows("value_output", value_output, shape, dtype, device)
     _native.check(
         _native.launch().tf_paged_kv_read_token_q8(
             cache.key.data_ptr(), cache.value.data_ptr(), cache.key_scales.data_ptr(),
@@ -322,8 +329,10 @@ def paged_gqa_decode_attention_q8(
         held = 1 << 30
     else:
         partials = (workspace.partial_max, workspace.partial_sum, workspace.partial_accumulator)
-        if (any(t.device != device or t.dtype != torch.float32 or not t.is_contiguous() for t in partials)
-                or workspace.partial_accumulator.ndim != 2 or workspace.partial_accumulator.shape[1] < head_dim):
+        for partial in partials:
+            if partial.device != device or partial.dtype != torch.float32 or not partial.is_contiguous():
+                raise ValueError("split-KV workspace has insufficient or incompatible capacity")
+        if partials[2].ndim != 2 or partials[2].shape[1] < head_dim:
             raise ValueError("split-KV workspace has insufficient or incompatible capacity")
         held = min(partials[0].numel(), partials[1].numel(), partials[2].shape[0])
     split_size, num_splits = attention_q8_plan(launch_context, batch, kv_heads, held // programs)
@@ -337,7 +346,7 @@ def paged_gqa_decode_attention_q8(
             maximum = accumulator + 4 * held * stride
             total = maximum + 4 * held
         else:
-            stride = workspace.partial_accumulator.shape[1]
+            stride = partials[2].shape[1]
             maximum, total, accumulator = (t.data_ptr() for t in partials)
     _native.check(
         _native.launch().tf_paged_gqa_decode_q8(
