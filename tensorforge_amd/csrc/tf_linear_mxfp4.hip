@@ -104,6 +104,50 @@ __host__ __device__ constexpr int scale_pitch(int32_t k) {
   return 4 * ((bytes + 3) / 4 | 1);
 }
 
+// The scales of the tile's rows and of the columns [panel, end) to LDS.
+template <int NT>
+__device__ __forceinline__ void load_scales(const LinearParams &p, int32_t n0, int32_t panel, int32_t end,
+                                            unsigned char *scales, int scale_row) {
+  const int32_t bytes = (end - panel) / 32;
+  if (p.scale_words) {
+    const int32_t words = bytes / 4;
+    for (int32_t i = threadIdx.x; i < 16 * NT * words; i += blockDim.x) {
+      const int32_t row = i / words;
+      const int64_t from = min(n0 + row, p.n - 1) * p.scale_stride + panel / 32;
+      *reinterpret_cast<uint32_t *>(scales + row * scale_row + 4 * (i - row * words)) =
+          *reinterpret_cast<const uint32_t *>(p.scales + from + 4 * (i - row * words));
+    }
+  } else {
+    for (int32_t i = threadIdx.x; i < 16 * NT * bytes; i += blockDim.x) {
+      const int32_t row = i / bytes;
+      scales[row * scale_row + i - row * bytes] =
+          p.scales[min(n0 + row, p.n - 1) * p.scale_stride + panel / 32 + i - row * bytes];
+    }
+  }
+}
+
+// The wavefronts' sums [waves][MR][NT][64] added in their order, rounded and stored.
+template <typename T, int MR, int NT>
+__device__ __forceinline__ void join(const LinearParams &p, const f32x4 *sums, int waves, int32_t m0, int32_t n0) {
+  for (int item = threadIdx.x; item < MR * NT * 64; item += blockDim.x) {
+    f32x4 sum = sums[item];
+    for (int w = 1; w < waves; ++w) sum += sums[w * MR * NT * 64 + item];
+    const int32_t tile = item >> 6;
+    const int32_t r = m0 + 16 * (tile / NT) + (item & 15);
+    const int32_t first = n0 + 16 * (tile % NT) + 4 * ((item >> 4) & 3);
+    if (r >= p.m) continue;
+    T *out = static_cast<T *>(p.y) + r * p.y_stride;
+    const T *residual = p.residual ? static_cast<const T *>(p.residual) + r * p.residual_stride : nullptr;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (first + j >= p.n) break;
+      T value = from_float<T>(sum[j]);
+      if (residual) value = from_float<T>(to_float(value) + to_float(residual[first + j]));
+      out[first + j] = value;
+    }
+  }
+}
+
 // A workgroup computes a tile of 16 NT columns of y for 16 rows of x (XR of
 // which are loaded), over all of K.  Its wavefronts take the chunks of K in
 // turn, each through a ring of its own in LDS that direct-to-LDS loads fill,
@@ -251,22 +295,7 @@ __global__ void __launch_bounds__(512) linear_mxfp4_kernel(LinearParams p) {
 #pragma unroll
     for (int i = 0; i < STAGES; ++i)
       if (i < mine) load(base_of(i), i);
-    const int32_t bytes = (end - panel) / 32;
-    if (p.scale_words) {
-      const int32_t words = bytes / 4;
-      for (int32_t i = threadIdx.x; i < 16 * NT * words; i += blockDim.x) {
-        const int32_t row = i / words;
-        const int64_t from = min(n0 + row, p.n - 1) * p.scale_stride + panel / 32;
-        *reinterpret_cast<uint32_t *>(scales + row * scale_row + 4 * (i - row * words)) =
-            *reinterpret_cast<const uint32_t *>(p.scales + from + 4 * (i - row * words));
-      }
-    } else {
-      for (int32_t i = threadIdx.x; i < 16 * NT * bytes; i += blockDim.x) {
-        const int32_t row = i / bytes;
-        scales[row * scale_row + i - row * bytes] =
-            p.scales[min(n0 + row, p.n - 1) * p.scale_stride + panel / 32 + i - row * bytes];
-      }
-    }
+    load_scales<NT>(p, n0, panel, end, scales, scale_row);
     __syncthreads();
     int32_t c = 0;
     int stage = 0;
@@ -288,21 +317,192 @@ __global__ void __launch_bounds__(512) linear_mxfp4_kernel(LinearParams p) {
 #pragma unroll
   for (int t = 0; t < NT; ++t) sums[(wave * NT + t) * 64 + lane] = acc[t];
   __syncthreads();
-  for (int item = threadIdx.x; item < NT * 64; item += blockDim.x) {
-    f32x4 sum = sums[item];
-    for (int w = 1; w < waves; ++w) sum += sums[w * NT * 64 + item];
-    const int32_t r = m0 + (item & 15);
-    const int32_t first = n0 + 16 * (item >> 6) + 4 * ((item >> 4) & 3);
-    if (r >= p.m) continue;
-    T *out = static_cast<T *>(p.y) + r * p.y_stride;
-    const T *residual = p.residual ? static_cast<const T *>(p.residual) + r * p.residual_stride : nullptr;
+  join<T, 1, NT>(p, sums, waves, m0, n0);
+}
+
+// The same products for 17 to 64 rows and many columns: a workgroup computes all
+// 16 MR rows by 16 NT columns, so x is read once per 16 NT columns and not once
+// per row block and tile.  The eight wavefronts fill one ring together, each
+// takes an eighth of every chunk's columns for the whole tile, and a barrier a
+// chunk says that the chunk is there and that the buffer of the one before is
+// free.  A weight is decoded once for all rows.
+template <typename T, int MR, int NT, int STAGES>
+__global__ void __launch_bounds__(512) linear_mxfp4_rows_kernel(LinearParams p) {
+  typedef typename Operand<T>::V V;
+  constexpr int kWeightBytes = 2048 * NT;
+  constexpr int kStage = kWeightBytes + 8192 * MR;
+  constexpr int WAVES = 8;
+  constexpr int kWeightLoads = 2 * NT;  // of 1024 bytes: 8 rows of 128 bytes
+  constexpr int kMine = kWeightLoads / WAVES;
+  constexpr int kExtra = kWeightLoads % WAVES;  // wavefronts with one more
+  constexpr int kRowLoads = MR;                 // 2 rows of 512 bytes each
+  static_assert((kMine + 1 + kRowLoads) * (STAGES - 1) <= 63, "vmcnt range");
+  const int scale_row = scale_pitch(p.k);
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15;
+  const int quad = lane >> 4;
+  const int32_t n0 = static_cast<int32_t>(blockIdx.x) * 16 * NT;
+  unsigned char *scales = smem + STAGES * kStage;
+  const uint32_t lds0 = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char *)smem));
+  const bool extra = wave < kExtra;
+
+  // Piece i of row r at i ^ r, as above.
+  const uint8_t *weight[kMine + 1];
+  const int weight_piece = (lane & 7) ^ (lane >> 3);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (first + j >= p.n) break;
-      T value = from_float<T>(sum[j]);
-      if (residual) value = from_float<T>(to_float(value) + to_float(residual[first + j]));
-      out[first + j] = value;
+  for (int i = 0; i <= kMine; ++i)
+    weight[i] = p.weight +
+                static_cast<int64_t>(min(n0 + 8 * (wave + WAVES * i) + (lane >> 3), p.n - 1)) * p.weight_stride;
+  const T *x[kRowLoads];
+  int row_piece[kRowLoads];
+#pragma unroll
+  for (int i = 0; i < kRowLoads; ++i) {
+    const int row = 2 * (wave + WAVES * i) + (lane >> 5);
+    x[i] = static_cast<const T *>(p.x) + static_cast<int64_t>(min(row, p.m - 1)) * p.x_stride;
+    row_piece[i] = (lane & 31) ^ (row & 15);
+  }
+  auto load_weight = [&](int i, int32_t code, int stage) __attribute__((always_inline)) {
+    load_lds16<true>(weight[i] + code,
+                     __builtin_amdgcn_readfirstlane(lds0 + stage * kStage + (wave + WAVES * i) * 1024));
+  };
+  auto load = [&](int32_t base, int stage) __attribute__((always_inline)) {
+    const int32_t code = min(base / 2 + 16 * weight_piece, p.k / 2 - 16);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) load_weight(i, code, stage);
+    if (kExtra && extra) load_weight(kMine, code, stage);
+#pragma unroll
+    for (int i = 0; i < kRowLoads; ++i)
+      load_lds16(x[i] + min(base + 8 * row_piece[i], p.k - 8),
+                 __builtin_amdgcn_readfirstlane(lds0 + stage * kStage + kWeightBytes + (wave + WAVES * i) * 1024));
+  };
+
+  f32x4 acc[MR][NT];
+#pragma unroll
+  for (int r = 0; r < MR; ++r)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // This wavefront's products of a chunk: step `s` of group `piece`.
+  const int piece = 4 * (wave / 4) + quad;
+  const int s = wave % 4;
+
+  // The chunk at `base`, FLIGHT chunks having been issued behind it; then one
+  // more, at `next`, into the buffer of the chunk before.
+  auto multiply = [&](auto flight, int32_t base, int32_t panel, int stage, int32_t next) {
+    constexpr int kFlight = decltype(flight)::value;
+    if (kExtra && extra)
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"((kMine + 1 + kRowLoads) * kFlight) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"((kMine + kRowLoads) * kFlight) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+    if (next >= 0) load(next, stage == 0 ? STAGES - 1 : stage - 1);
+    const unsigned char *at = smem + stage * kStage;
+    uint32_t codes[NT], exponent[NT];
+    V rows[MR];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      codes[t] = *reinterpret_cast<const uint32_t *>(at + (16 * t + col) * 128 + 16 * (piece ^ (col & 7)) + 4 * s);
+      exponent[t] = scales[(16 * t + col) * scale_row + (base - panel) / 32 + piece];
     }
+#pragma unroll
+    for (int r = 0; r < MR; ++r)
+      rows[r] = *reinterpret_cast<const V *>(at + kWeightBytes + (16 * r + col) * 512 + 16 * ((4 * piece + s) ^ col));
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    if (base + kChunk > p.k && base + 32 * piece >= p.k) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        codes[t] = 0;
+        exponent[t] = 127;
+      }
+#pragma unroll
+      for (int r = 0; r < MR; ++r) rows[r] = V{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+    if constexpr (__is_same(T, _Float16)) {
+      bool wide = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) wide |= exponent[t] - (127 - 13) > 26;
+      if (__any(wide)) {
+#pragma unroll
+        for (int r = 0; r < MR; ++r) {
+          bf16x8 high, low;
+          split(rows[r], high, low);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            asm volatile("" : "+v"(codes[t]));  // decoded again: the decoded weights would not fit beside the sums
+            const bf16x8 a = Operand<__bf16>::decode(codes[t], __builtin_bit_cast(float, exponent[t] << 23));
+            acc[r][t] = Operand<__bf16>::mfma(a, high, acc[r][t]);
+            acc[r][t] = Operand<__bf16>::mfma(a, low, acc[r][t]);
+          }
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const V a = Operand<T>::decode(codes[t], __builtin_bit_cast(float, exponent[t] << 23));
+#pragma unroll
+      for (int r = 0; r < MR; ++r) acc[r][t] = Operand<T>::mfma(a, rows[r], acc[r][t]);
+    }
+  };
+
+  for (int32_t panel = 0; panel < p.k; panel += kPanel) {
+    const int32_t end = min(panel + kPanel, p.k);
+    const int32_t chunks = (end - panel + kChunk - 1) / kChunk;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+      if (i < chunks) load(panel + i * kChunk, i);
+    load_scales<NT>(p, n0, panel, end, scales, scale_row);
+    __syncthreads();
+    int32_t c = 0;
+    int stage = 0;
+    auto step = [&](auto flight, bool more) {
+      multiply(flight, panel + c * kChunk, panel, stage, more ? panel + (c + STAGES - 1) * kChunk : -1);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      ++c;
+    };
+    while (c + STAGES - 1 < chunks) step(std::integral_constant<int, STAGES - 2>{}, true);
+    if constexpr (STAGES >= 3)
+      if (chunks - c >= 2) step(std::integral_constant<int, 1>{}, false);
+    if (chunks - c >= 1) step(std::integral_constant<int, 0>{}, false);
+    __syncthreads();  // the panel's scales and the ring are done with
+  }
+
+  // The upper four wavefronts' sums go to the lower ones.
+  f32x4 *sums = reinterpret_cast<f32x4 *>(smem);  // [4][MR][NT][64]
+  f32x4 *mine = sums + wave % 4 * MR * NT * 64 + lane;
+  if (wave >= 4) {
+#pragma unroll
+    for (int r = 0; r < MR; ++r)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) mine[(r * NT + t) * 64] = acc[r][t];
+  }
+  __syncthreads();
+  if (wave < 4) {
+#pragma unroll
+    for (int r = 0; r < MR; ++r)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) mine[(r * NT + t) * 64] += acc[r][t];
+  }
+  __syncthreads();
+  join<T, MR, NT>(p, sums, 4, 0, n0);
+}
+
+// Raise a kernel's dynamic LDS limit once per device (a failure shows up as a
+// launch error).
+template <auto KERNEL>
+void raise_lds(size_t lds) {
+  if (lds <= 64 * 1024) return;
+  constexpr int kMaxDevices = 64;
+  static std::atomic<bool> raised[kMaxDevices];
+  int device = 0;
+  if (hipGetDevice(&device) == hipSuccess && device >= 0 && device < kMaxDevices &&
+      !raised[device].load(std::memory_order_acquire)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize,
+                            160 * 1024) == hipSuccess)
+      raised[device].store(true, std::memory_order_release);
   }
 }
 
@@ -310,22 +510,10 @@ template <typename T, int XR, int NT>
 int32_t launch_linear(LinearParams p, int waves, hipStream_t stream) {
   constexpr int stage = 1024 * (2 * NT + XR / 2);
   auto kernel = linear_mxfp4_kernel<T, XR, NT>;
-  const size_t ring = static_cast<size_t>(waves) * ring_stages(stage) * stage + 16 * NT * scale_pitch(p.k);
+  const size_t ring = static_cast<size_t>(waves) * ring_stages(stage) * stage + 16 * NT * scale_pitch(p.k) + 8;
   const size_t sums = static_cast<size_t>(waves) * NT * 64 * sizeof(f32x4);
   const size_t lds = ring > sums ? ring : sums;
-  if (lds > 64 * 1024) {
-    // Raise the kernel's dynamic LDS limit once per device (a failure shows
-    // up as a launch error).
-    constexpr int kMaxDevices = 64;
-    static std::atomic<bool> raised[kMaxDevices];
-    int device = 0;
-    if (hipGetDevice(&device) == hipSuccess && device >= 0 && device < kMaxDevices &&
-        !raised[device].load(std::memory_order_acquire)) {
-      if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                              160 * 1024) == hipSuccess)
-        raised[device].store(true, std::memory_order_release);
-    }
-  }
+  raise_lds<linear_mxfp4_kernel<T, XR, NT>>(lds);
   p.column_tiles = (p.n + 16 * NT - 1) / (16 * NT);
   p.row_blocks = (p.m + 15) / 16;
   const unsigned grid = static_cast<unsigned>((p.column_tiles + kXcds - 1) / kXcds * kXcds) * p.row_blocks;
@@ -352,8 +540,7 @@ int32_t launch_columns(const LinearParams &p, int tiles, int waves, hipStream_t 
 // of NT 1 to 4 with 2, 4 and 8 wavefronts against the choice (us): 1 row of
 // 2048 x 5632 5.3 / 5.3, 8 of 28672 x 4096 15.6 / 16.6, 16 of 32000 x 2048
 // 11.8 / 11.8, 16 of 4096 x 14336 15.0 / 15.0, 32 of 11264 x 2048 8.5 / 8.5,
-// 64 of 2048 x 2048 5.2 / 5.2, 64 of 4096 x 4096 10.3 / 10.4, 64 of 11264 x
-// 2048 13.5 / 14.4.
+// 64 of 2048 x 2048 5.2 / 5.2, 64 of 4096 x 4096 10.3 / 10.4.
 constexpr int64_t kUnits = 256;
 
 void choose_tile(const LinearParams &p, int loaded_rows, int &tiles, int &waves) {
@@ -379,17 +566,69 @@ int32_t launch_tile(const LinearParams &p, hipStream_t stream) {
   return launch_columns<T, XR>(p, tiles, waves, stream);
 }
 
+// All rows in a workgroup: from kWideColumns columns, where 256 workgroups of
+// three operands' columns are filled, tiles as wide as one round of 256 needs.
+// Three chunks in the ring, two where LDS does not hold three.  Measured against
+// the tiles of 16 rows (us): 64 rows of 11264 x 2048 15.4 / 11.9, of 16384 x
+// 4096 29.7 / 19.2, of 28672 x 4096 48.6 / 28.5, of 32000 x 2048 30.9 / 21.2,
+// of 64000 x 1024 39.6 / 29.2, of 8704 x 14336 55.2 / 47.6; 40 rows of 28672 x
+// 4096 39.9 / 24.0; 32 rows of 11264 x 2048 8.7 / 9.3, of 28672 x 4096 29.7 /
+// 23.4; below, 64 rows of 4096 x 4096 10.4 / 10.6, of 2048 x 2048 5.4 / 7.0.
+// 64 rows of 16384 x 4096 with 4 / 8 wavefronts 21.5 / 19.2.
+constexpr int32_t kWideColumns = 8192;
+
+template <typename T, int MR, int NT, int STAGES>
+int32_t launch_wide_stages(const LinearParams &p, size_t lds, hipStream_t stream) {
+  constexpr auto kernel = linear_mxfp4_rows_kernel<T, MR, NT, STAGES>;
+  raise_lds<kernel>(lds);
+  hipLaunchKernelGGL(kernel, dim3((p.n + 16 * NT - 1) / (16 * NT)), dim3(512), lds, stream, p);
+  return check_launch("linear_mxfp4");
+}
+
+template <typename T, int MR, int NT>
+int32_t launch_wide_tile(const LinearParams &p, hipStream_t stream) {
+  constexpr size_t stage = 2048 * NT + 8192 * MR;
+  const size_t scales = 16 * NT * scale_pitch(p.k) + 8;
+  constexpr size_t sums = 4 * MR * NT * 64 * sizeof(f32x4);
+  const auto lds = [&](size_t stages) { return stages * stage + scales > sums ? stages * stage + scales : sums; };
+  if (lds(3) <= 160 * 1024) return launch_wide_stages<T, MR, NT, 3>(p, lds(3), stream);
+  return launch_wide_stages<T, MR, NT, 2>(p, lds(2), stream);
+}
+
+// fp16 has the second path for weights past its range, with which the sums of
+// more than 21 tiles do not stay in registers: wider calls then take tiles of
+// four operands' columns (64 rows of 28672 x 4096 43.7 us).
+template <typename T, int MR>
+int32_t launch_wide(const LinearParams &p, hipStream_t stream) {
+  constexpr int kMost = __is_same(T, _Float16) ? 21 / MR : 8;
+  const int64_t width = (p.n + 16 * kUnits - 1) / (16 * kUnits);
+  if (width == 3) return launch_wide_tile<T, MR, 3>(p, stream);
+  if (width == 5) return launch_wide_tile<T, MR, 5>(p, stream);
+  if constexpr (kMost >= 6)
+    if (width == 6) return launch_wide_tile<T, MR, 6>(p, stream);
+  if constexpr (kMost >= 7)
+    if (width == 7) return launch_wide_tile<T, MR, 7>(p, stream);
+  if constexpr (kMost >= 8)
+    if (width >= 8) return launch_wide_tile<T, MR, 8>(p, stream);
+  return launch_wide_tile<T, MR, 4>(p, stream);
+}
+
 template <typename T>
 int32_t launch_rows(const LinearParams &p, hipStream_t stream) {
   if (p.m <= 2) return launch_tile<T, 2>(p, stream);
   if (p.m <= 4) return launch_tile<T, 4>(p, stream);
   if (p.m <= 8) return launch_tile<T, 8>(p, stream);
+  if (p.m > 16 && p.n > kWideColumns) {
+    if (p.m <= 32) return launch_wide<T, 2>(p, stream);
+    if (p.m <= 48) return launch_wide<T, 3>(p, stream);
+    return launch_wide<T, 4>(p, stream);
+  }
   return launch_tile<T, 16>(p, stream);
 }
 
 // Bytes of codes from which weights that several row blocks read pass the
-// caches by (64 rows of 2048 x 5632 cached 8.0 us, past 8.8; of 11264 x 2048
-// 14.4 and 13.5); one row block always does (1 row of 2048 x 2048 4.0 and 3.8).
+// caches by (64 rows of 2048 x 5632 cached 8.0 us, past 8.8; in these tiles, of
+// 11264 x 2048 14.4 and 13.5); one row block always does (1 row of 2048 x 2048 4.0 and 3.8).
 constexpr int64_t kCached = 8000000;
 
 }  // namespace

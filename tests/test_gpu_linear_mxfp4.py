@@ -53,6 +53,42 @@ def test_shapes(device, dtype, m, n, k):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize(("m", "n", "k"), [
+    (17, 8193, 32), (32, 12300, 288), (33, 16385, 96), (48, 20481, 544), (49, 24577, 256), (64, 28673, 160),
+    (64, 40001, 800), (40, 8200, 8224)])
+def test_many_columns(device, dtype, m, n, k):
+    """All rows in one workgroup: every width of its tiles, K behind a chunk, a ring and a panel of scales."""
+
+    generator = torch.Generator().manual_seed(m + n + k)
+    x = torch.randn(m, k + 8, generator=generator).to(dtype)[:, :k]
+    codes = torch.randint(0, 256, (n, k // 2), generator=generator, dtype=torch.uint8)
+    scales = torch.randint(118, 124, (n, k // 32), generator=generator, dtype=torch.uint8)
+    if dtype == torch.float16:
+        scales[::37, 0] = 100  # weights that fp16 cannot hold
+    scales = scales.view(torch.float8_e8m0fnu)
+    residual = torch.randn(m, n, generator=generator).to(dtype)
+    buffer = torch.full((m + 2, n + 3), 7, dtype=dtype, device=device)
+    rows = torch.empty(m, k + 8, dtype=dtype, device=device)[:, :k].copy_(x)
+    got = linear_mxfp4(rows, *_on(device, codes, scales), residual=residual.to(device), output=buffer[1:-1, :n])
+    _check(got, *linear(x, codes, scales, residual))
+    assert (buffer[0] == 7).all() and (buffer[-1] == 7).all() and (buffer[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_columns_keep_values_that_are_not_finite_in_their_rows(device, dtype):
+    m, n, k = 50, 8400, 320
+    x, codes, scales, _ = _inputs(m, n, k, dtype, seed=3)
+    clean = linear_mxfp4(x.to(device), *_on(device, codes, scales))
+    bad = x.clone()
+    bad[7, 300] = torch.nan
+    bad[49, 0] = torch.inf
+    got = linear_mxfp4(bad.to(device), *_on(device, codes, scales))
+    assert torch.isnan(got[7]).all() and not torch.isfinite(got[49]).any()
+    keep = [r for r in range(m) if r not in (7, 49)]
+    assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_every_code_in_every_place(device, dtype):
     """One-hot rows read single weights back exactly, for all 16 codes in every
     column of a group and scales far apart."""
