@@ -15,7 +15,8 @@
 // Operands go through LDS.  Loaded in the operand layout (16 rows of 64 bytes
 // an instruction, a scale byte from each) the same products were bound by the
 // 53 B/ns at which a compute unit takes lines: 8 rows by 28672 x 4096 24 us,
-// 64 by 2048 x 2048 11 us.
+// 64 by 2048 x 2048 11 us; through LDS 15.7 and 5.2.  At few rows HBM bounds
+// (8 by 28672 x 4096 reads 4.0 TB/s), at many that rate still: x for every tile.
 #include <atomic>
 #include <type_traits>
 
@@ -644,6 +645,7 @@ extern "C" int32_t tf_linear_mxfp4(const void *x, int64_t x_row_stride, const vo
     return fail(TF_ERROR_UNSUPPORTED, "linear_mxfp4 takes fp16 or bf16 activations");
   if (m < 0 || m > kMaxRows || n < 0 || k <= 0 || k % 32 != 0)
     return fail(TF_ERROR_INVALID_ARGUMENT, "linear_mxfp4 takes at most 64 rows and a K that is a multiple of 32");
+  if (n > 1 << 28 || k > 1 << 28) return fail(TF_ERROR_UNSUPPORTED, "linear_mxfp4 takes at most 2^28 columns and K");
   if (m == 0 || n == 0) return TF_SUCCESS;
   if (!x || !weight || !scales || !y) return fail(TF_ERROR_INVALID_ARGUMENT, "null tensor pointer");
   if (x_row_stride < k || weight_row_stride < k / 2 || scale_row_stride < k / 32 || y_row_stride < n ||

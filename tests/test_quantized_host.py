@@ -151,6 +151,15 @@ def test_c_abi_refusals(call, changed, status, message):
     assert message in library.tf_last_error().decode()
 
 
+@pytest.mark.parametrize("changed", [
+    {"n": (1 << 28) + 1, "y_stride": 1 << 29},
+    {"k": (1 << 28) + 32, "x_stride": 1 << 29, "weight_stride": 1 << 28, "scale_stride": 1 << 24}])
+def test_projections_past_32_bit_indexes_are_refused(changed):
+    library = _native.library()
+    assert _project(library, **changed) == 2
+    assert "2^28" in library.tf_last_error().decode()
+
+
 def test_c_abi_calls_without_rows_do_nothing():
     library = _native.library()
     assert _write(library, rows=0, keys=None, values=None, blocks=None, offsets=None, active=None) == 0
