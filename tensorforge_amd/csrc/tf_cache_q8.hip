@@ -138,7 +138,9 @@ __device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_A
 
 // One workgroup per (`count` rows, kv head): wavefront 0 stores the keys of the
 // runs that start in them, wavefront 1 the values.  Per element (lanes across
-// dimensions, two bytes in and one out) 8,058 rows at 4 heads of 64 took 14.6 us.
+// dimensions, two bytes in and one out) 8,058 rows at 4 heads of 64 took 14.6 us,
+// by pieces 7.1 (12.4 MB, 2.2 of it an empty launch): latency of a run's scale,
+// rows and stores, one run of a workgroup after the other.
 template <typename T, int PER>
 __global__ void __launch_bounds__(128)
 kv_write_q8_kernel(const T *__restrict__ keys, const T *__restrict__ values, uint8_t *__restrict__ key_cache,
@@ -234,7 +236,8 @@ kv_write_q8_kernel(const T *__restrict__ keys, const T *__restrict__ values, uin
   });
 }
 
-// The same split over workgroups; rows without a slot become zeros.
+// The same split over workgroups; rows without a slot become zeros.  8,058 rows
+// at 4 heads of 64 to bf16 11.3 us (12.4 MB).
 template <typename T, int PER>
 __global__ void __launch_bounds__(128)
 kv_read_q8_kernel(const uint8_t *__restrict__ key_cache, const uint8_t *__restrict__ value_cache,

