@@ -567,7 +567,7 @@ int32_t launch_tile(const LinearParams &p, hipStream_t stream) {
   return launch_columns<T, XR>(p, tiles, waves, stream);
 }
 
-// All rows in a workgroup: from kWideColumns columns, where 256 workgroups of
+// All rows in a workgroup: above kWideColumns columns, where 256 workgroups of
 // three operands' columns are filled, tiles as wide as one round of 256 needs.
 // Three chunks in the ring, two where LDS does not hold three.  Measured against
 // the tiles of 16 rows (us): 64 rows of 11264 x 2048 15.4 / 11.9, of 16384 x
